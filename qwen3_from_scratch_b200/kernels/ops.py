@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -79,6 +79,16 @@ _SIGNATURES = {
                         _c_void_p],
     "q3_attn_tc": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int,
                    _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_void_p, _c_void_p],
+    "q3_fp4_quantise": [_c_void_p, _c_int, _c_ll, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p],
+    "q3_fp4_add_rmsnorm": [_c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_float,
+                           _c_void_p],
+    "q3_fp4_product": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_ll, _c_int, _c_void_p,
+                       _c_void_p],
+    "q3_fp4_gated_product": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int,
+                             _c_void_p, _c_void_p],
+    "q3_fp4_feed_forward": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_float, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                            _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
+                            _c_void_p, _c_void_p],
     "q3_swiglu": [_c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_void_p],
     "q3_gemm_tc": [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p,
                    _c_void_p],
@@ -233,7 +243,8 @@ _SIGNATURES = {
 }
 
 
-_WAIT_TEST = ("q3_gemm_tc_wait_test", "q3_attn_tc_wait_test", "q3_attn_decode_tma_wait_test", "q3_latent_attn_tc_wait_test")
+_WAIT_TEST = ("q3_gemm_tc_wait_test", "q3_attn_tc_wait_test", "q3_attn_decode_tma_wait_test", "q3_latent_attn_tc_wait_test",
+              "q3_gemm_fp4_wait_test")
 
 
 def library() -> ctypes.CDLL:
@@ -3127,3 +3138,155 @@ def rotate_columns(x: torch.Tensor, column: int, heads: int, dim: int, dims: int
     code = library().q3_rotate_columns(x.data_ptr(), ld, int(column), int(heads), int(dim), int(dims), freq.data_ptr(),
                                        float(magnitude), positions.data_ptr(), dtype_tag(x.dtype), T, _stream())
     _done("rotate_columns", code, f"rotated {dims} of {dim}")
+
+
+# ------------------------------------------------------------------ rows held in microscaled 4-bit floating point
+FP4_BLOCK = 32             # values of a row that share a scale
+FP4_MAX_NORM_WIDTH = 32768  # widest row of fp4_add_rmsnorm
+FP4_GATES = ("silu", "relu", "gelu_tanh")
+
+
+class Fp4Rows(NamedTuple):
+    """Rows of ``width`` values in microscaled 4-bit floating point: a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 per value,
+    and a power-of-two scale 2^(b - 127) per block of 32 values of a row.
+
+    ``codes``: uint8 [rows, 16 ceil(width / 32)], value 2 i in the low half of byte i; zeros beyond the width.
+    ``scales``: uint8, tiles of 128 rows x 4 blocks, [at least ceil(rows / 128), ceil(width / 128), 512]: the byte b of row r,
+    block j is byte 16 (r % 32) + 4 ((r % 128) / 32) + j % 4 of tile (r / 128, j / 4); zeros beyond the width.  255 is NaN."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    width: int
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+    def first(self, rows: int) -> "Fp4Rows":
+        """The first ``rows`` rows, in the same memory."""
+        return Fp4Rows(self.codes[:rows], self.scales, self.width)
+
+
+def fp4_rows(rows: int, width: int, device) -> Fp4Rows:
+    """Memory for that many rows, zeroed."""
+    if rows < 0 or width <= 0:
+        raise KernelSizeError(f"fp4_rows: {rows} rows of {width} values")
+    return Fp4Rows(torch.zeros(rows, -(-width // FP4_BLOCK) * 16, dtype=torch.uint8, device=device),
+                   torch.zeros(-(-rows // 128), -(-width // 128), 512, dtype=torch.uint8, device=device), width)
+
+
+def _check_fp4(name: str, r: Fp4Rows, width: Optional[int] = None, rows: Optional[int] = None) -> None:
+    _check(f"{name}.codes", r.codes, torch.uint8)
+    _check(f"{name}.scales", r.scales, torch.uint8)
+    n, tiles = r.codes.shape[0], r.scales.shape
+    if (r.width <= 0 or r.codes.dim() != 2 or r.codes.shape[1] != (r.width + 31) // 32 * 16 or len(tiles) != 3
+            or tiles[0] < (n + 127) // 128 or tiles[1] != (r.width + 127) // 128 or tiles[2] != 512):
+        raise KernelError(f"{name}: rows of {r.width} values do not have codes {tuple(r.codes.shape)} and scales {tuple(tiles)}")
+    if (width is not None and r.width != width) or (rows is not None and n != rows):
+        raise KernelError(f"{name}: {n} rows of {r.width} values, expected {n if rows is None else rows} of "
+                          f"{r.width if width is None else width}")
+
+
+def fp4_quantise(x: torch.Tensor, out: Fp4Rows, values: Optional[torch.Tensor] = None) -> None:
+    """Rounds the rows of x [T, K] (float32 or bfloat16; rows may lie further apart than K) into ``out``.  A block's scale is the
+    smallest power of two X with max|x| <= 7 X; each x / X goes to the nearest value of the format, ties to the even code, and to
+    +-6 beyond it.  A block that holds a value that is not finite gets the scale NaN.  ``values`` (float32 or bfloat16 [T, K],
+    contiguous): what the rows then stand for, exact in either type."""
+    if not x.is_cuda:
+        raise KernelError(f"fp4_quantise.x: tensor is on {x.device}; the kernels run on the GPU only")
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or x.stride(0) < 0:
+        raise KernelError(f"fp4_quantise.x: rows of contiguous values wanted, got shape {tuple(x.shape)}, strides {x.stride()}")
+    T, K = x.shape
+    _check_fp4("fp4_quantise.out", out, K, T)
+    tag = dtype_tag(x.dtype)
+    if values is not None:
+        _check("fp4_quantise.values", values)
+        if tuple(values.shape) != (T, K):
+            raise KernelError(f"fp4_quantise: values {tuple(values.shape)}, x {(T, K)}")
+    code = library().q3_fp4_quantise(x.data_ptr(), tag, x.stride(0), out.codes.data_ptr(), out.scales.data_ptr(), _ptr(values),
+                                     tag if values is None else dtype_tag(values.dtype), T, K, _stream())
+    _done("fp4_quantise", code, f"{T} rows of {K}")
+
+
+def _check_fp4_stream(name: str, stream: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor,
+                      stream_out: Optional[torch.Tensor], dtype: torch.dtype) -> Tuple[int, int]:
+    _check(f"{name}.stream", stream, torch.float32)
+    _check(f"{name}.weight", weight, torch.float32)
+    T, H = stream.shape
+    if delta is not None:
+        _check(f"{name}.delta", delta, dtype)
+        if tuple(delta.shape) != (T, H):
+            raise KernelError(f"{name}: delta {tuple(delta.shape)} vs stream {(T, H)}")
+    if stream_out is not None:
+        _check(f"{name}.stream_out", stream_out, torch.float32)
+        if tuple(stream_out.shape) != (T, H):
+            raise KernelError(f"{name}: stream_out {tuple(stream_out.shape)} vs stream {(T, H)}")
+    if weight.numel() != H:
+        raise KernelError(f"{name}: weight {tuple(weight.shape)}, stream {(T, H)}")
+    return T, H
+
+
+def fp4_add_rmsnorm(stream: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, out: Fp4Rows, eps: float,
+                    stream_out: Optional[torch.Tensor] = None) -> None:
+    """s = stream + delta (when given) goes to ``stream_out`` (None: the stream itself); out = the rows of rmsnorm(s) * weight, as
+    ``fp4_quantise`` rounds them, from float32.  Rows of up to ``FP4_MAX_NORM_WIDTH`` values."""
+    T, H = _check_fp4_stream("fp4_add_rmsnorm", stream, delta, weight, stream_out, torch.float32 if delta is None else delta.dtype)
+    _check_fp4("fp4_add_rmsnorm.out", out, H, T)
+    code = library().q3_fp4_add_rmsnorm(stream.data_ptr(), _ptr(delta), F32 if delta is None else dtype_tag(delta.dtype),
+                                        weight.data_ptr(), (stream if stream_out is None else stream_out).data_ptr(),
+                                        out.codes.data_ptr(), out.scales.data_ptr(), T, H, float(eps), _stream())
+    _done("fp4_add_rmsnorm", code, f"width {H}")
+
+
+def fp4_product(x: Fp4Rows, w: Fp4Rows, out: torch.Tensor, status: torch.Tensor) -> None:
+    """out[T, N] = x[T, K] @ w[N, K]^T of rows held in four bits, accumulated in float32; out bfloat16 or float32, also a column
+    view of a wider buffer."""
+    _check_fp4("fp4_product.x", x)
+    _check_fp4("fp4_product.w", w, x.width)
+    T, N = x.rows, w.rows
+    if not out.is_cuda or out.dim() != 2 or tuple(out.shape) != (T, N) or (N > 1 and out.stride(1) != 1) or (T > 1 and out.stride(0) < N):
+        raise KernelError(f"fp4_product: out {tuple(out.shape)} with strides {out.stride()} on {out.device} for {T} x {N}")
+    code = library().q3_fp4_product(x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
+                                    T, N, x.width, max(out.stride(0), N), 1 if dtype_tag(out.dtype) == F32 else 0,
+                                    status.data_ptr(), _stream())
+    _done("fp4_product", code, f"T {T} N {N} K {x.width}")
+
+
+def _fp4_gate(name: str, activation: str) -> int:
+    if activation not in FP4_GATES:
+        raise KernelError(f"{name}: no gate {activation!r} (there are {FP4_GATES})")
+    return activation_code(activation, gate=True)
+
+
+def fp4_gated_product(x: Fp4Rows, w: Fp4Rows, out: Fp4Rows, status: torch.Tensor, activation: str = "silu") -> None:
+    """out = the rows of act(gate) * up, rounded as by ``fp4_quantise`` from float32: w's 2 I rows alternate gate/up in blocks
+    of eight (I a multiple of 8), gate and up are the products of x with them."""
+    _check_fp4("fp4_gated_product.x", x)
+    _check_fp4("fp4_gated_product.w", w, x.width)
+    _check_fp4("fp4_gated_product.out", out, w.rows // 2, x.rows)
+    code = library().q3_fp4_gated_product(x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(),
+                                          out.codes.data_ptr(), out.scales.data_ptr(), x.rows, w.rows, x.width,
+                                          _fp4_gate("fp4_gated_product", activation), status.data_ptr(), _stream())
+    _done("fp4_gated_product", code, f"T {x.rows} N {w.rows} K {x.width}")
+
+
+def fp4_feed_forward(stream: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, eps: float, gate_up: Fp4Rows,
+                     down: Fp4Rows, normed: Fp4Rows, gated: Fp4Rows, out: torch.Tensor, status: torch.Tensor,
+                     activation: str = "silu", stream_out: Optional[torch.Tensor] = None) -> None:
+    """A gated feed-forward behind its norm in one call: ``fp4_add_rmsnorm`` into ``normed`` [T, H], ``fp4_gated_product``
+    with ``gate_up`` [2 I, H] into ``gated`` [T, I], and out[T, H] = gated @ down[H, I]^T; delta has the dtype of out."""
+    _check("fp4_feed_forward.out", out)
+    T, H = _check_fp4_stream("fp4_feed_forward", stream, delta, weight, stream_out, out.dtype)
+    inner = down.width
+    _check_fp4("fp4_feed_forward.gate_up", gate_up, H, 2 * inner)
+    _check_fp4("fp4_feed_forward.down", down, inner, H)
+    _check_fp4("fp4_feed_forward.normed", normed, H, T)
+    _check_fp4("fp4_feed_forward.gated", gated, inner, T)
+    if tuple(out.shape) != (T, H):
+        raise KernelError(f"fp4_feed_forward: out {tuple(out.shape)} vs stream {(T, H)}")
+    code = library().q3_fp4_feed_forward(
+        stream.data_ptr(), _ptr(delta), weight.data_ptr(), (stream if stream_out is None else stream_out).data_ptr(), float(eps),
+        gate_up.codes.data_ptr(), gate_up.scales.data_ptr(), down.codes.data_ptr(), down.scales.data_ptr(),
+        normed.codes.data_ptr(), normed.scales.data_ptr(), gated.codes.data_ptr(), gated.scales.data_ptr(), out.data_ptr(),
+        dtype_tag(out.dtype), T, H, inner, _fp4_gate("fp4_feed_forward", activation), status.data_ptr(), _stream())
+    _done("fp4_feed_forward", code, f"T {T} H {H} I {inner}")

@@ -1,0 +1,378 @@
+"""Rows in microscaled 4-bit floating point and the products of such rows, against the definition in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+import plain_fp4 as plain
+
+pytestmark = pytest.mark.gpu
+
+DT = {"float32": torch.float32, "bfloat16": torch.bfloat16}
+
+
+def ops():
+    from qwen3_from_scratch_b200.kernels import ops as o
+    return o
+
+
+def status():
+    return torch.zeros(1, dtype=torch.int32, device="cuda")
+
+
+def normal(rows, width, seed, spread=True):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, width, generator=g)
+    return x * torch.exp(0.7 * torch.randn(width, generator=g)) if spread else x
+
+
+def held(x):
+    """The rows of a CPU tensor, rounded on the GPU, and what they stand for in float64."""
+    o = ops()
+    r = o.fp4_rows(x.shape[0], x.shape[1], "cuda")
+    o.fp4_quantise(x.cuda(), r)
+    return r, plain.read(r.codes, r.scales, x.shape[1])[0]
+
+
+def junk_rows(rows, width):
+    """Memory for rows with every byte set: what a kernel does not write stays visible."""
+    r = ops().fp4_rows(rows, width, "cuda")
+    r.codes.fill_(0xA5)
+    r.scales.fill_(0xFF)
+    return r
+
+
+def pad_is_zero(r):
+    """Codes beyond the width and the scales of blocks beyond it."""
+    rows, k = r.codes.shape[0], r.width
+    nibbles = torch.stack([r.codes & 15, r.codes >> 4], dim=-1).reshape(rows, -1).cpu()
+    across = r.scales.shape[1]
+    _, byte = plain.read(torch.zeros(rows, across * 64, dtype=torch.uint8), r.scales, across * 128)
+    return bool((nibbles[:, k:] == 0).all()) and bool((byte[:, -(-k // 32):] == 0).all())
+
+
+# ---------------------------------------------------------------- rounding
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("rows,width", [(1, 1), (1, 31), (1, 32), (3, 33), (2, 127), (5, 128), (4, 129), (2, 256), (130, 264),
+                                        (129, 300), (7, 1000), (3, 4104), (257, 96), (1, 12288)])
+def test_quantise(dtype, rows, width):
+    x = normal(rows, width, rows * 10007 + width).to(DT[dtype])
+    r = junk_rows(rows, width)
+    values = torch.empty(rows, width, dtype=torch.float32, device="cuda")
+    ops().fp4_quantise(x.cuda(), r, values=values)
+    want = plain.rounded(x.double())
+    got, _ = plain.read(r.codes, r.scales, width)
+    assert torch.equal(got, want)  # rounding is exact: no tolerance
+    assert torch.equal(values.cpu().double(), want)
+    assert pad_is_zero(r)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("pitch,start", [(300, 0), (301, 0), (304, 8), (333, 1), (320, 3)])
+def test_quantise_columns_of_a_wider_buffer(dtype, pitch, start):
+    wide = normal(9, pitch, pitch).to(DT[dtype])
+    width = 290
+    x = wide.cuda()[:, start:start + width]
+    r = junk_rows(9, width)
+    values = torch.empty(9, width, dtype=torch.bfloat16, device="cuda")
+    ops().fp4_quantise(x, r, values=values)
+    want = plain.rounded(wide[:, start:start + width].double())
+    assert torch.equal(plain.read(r.codes, r.scales, width)[0], want)
+    assert torch.equal(values.cpu().double(), want)
+
+
+def test_quantise_ties_ends_and_signs():
+    """Every boundary between two codes at several scales, the values around the boundary between two scales, zeros of both
+    signs, the smallest and the largest floats."""
+    rows = []
+    for e in (-126, -100, -3, 0, 40, 120):
+        unit = 2.0 ** e
+        row = [s * m * unit for m in (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 6.5) for s in (1, -1)]
+        rows.append(row + [7.0 * unit] + [0.0] * (32 - len(row) - 1))
+        rows.append(row + [math.nextafter(7.0, 8.0) * unit * (1 + 2.0 ** -22)] + [-0.0] * (32 - len(row) - 1))
+    rows += [[0.0] * 32, [-0.0] * 32, [2.0 ** -149] * 32, [2.0 ** -127, -(2.0 ** -128)] * 16, [2.0 ** -126 * 1.75] * 32]
+    x = torch.tensor(rows, dtype=torch.float64).float()
+    assert bool(torch.isfinite(x).all())
+    r = junk_rows(x.shape[0], 32)
+    ops().fp4_quantise(x.cuda(), r)
+    got, byte = plain.read(r.codes, r.scales, 32)
+    assert torch.equal(got, plain.rounded(x.double()))
+    assert torch.equal(byte[:, 0].int() - 127, plain.scale_exponents(x.double())[:, 0])
+    big = torch.full((1, 32), torch.finfo(torch.float32).max).cuda()
+    b = junk_rows(1, 32)
+    ops().fp4_quantise(big, b)  # the largest float has a scale of its own; its value rounds up to 4 x 2^126
+    assert int(b.scales.reshape(-1)[0]) == 253 and bool((b.codes == 0x66).all())
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_quantise_what_is_not_finite(bad):
+    x = normal(3, 100, 5)
+    x[1, 40] = bad
+    r = junk_rows(3, 100)
+    values = torch.empty(3, 100, device="cuda")
+    ops().fp4_quantise(x.cuda(), r, values=values)
+    clean = x.clone()
+    clean[1, 32:64] = 0
+    want = plain.rounded(clean.double())
+    want[1, 32:64] = math.nan
+    assert torch.equal(values.cpu().double().nan_to_num(77.0), want.nan_to_num(77.0))
+    assert torch.equal(plain.read(r.codes, r.scales, 100)[0].nan_to_num(77.0), want.nan_to_num(77.0))
+
+
+# ---------------------------------------------------------------- the norm
+@pytest.mark.parametrize("dtype", [None, "float32", "bfloat16"])
+@pytest.mark.parametrize("rows,width", [(1, 8), (2, 33), (5, 1000), (130, 264), (3, 4096), (2, 5121), (2, 12288), (1, 32768)])
+def test_add_rmsnorm(dtype, rows, width):
+    stream = normal(rows, width, 3 * rows + width) * 2
+    delta = None if dtype is None else (normal(rows, width, 7 * width) * 0.3).to(DT[dtype])
+    w = 1 + 0.1 * normal(1, width, 11, spread=False)[0]
+    total = stream if delta is None else stream + delta.float()
+    s = total.double()
+    h = s / torch.sqrt(s.square().mean(1, keepdim=True) + 1e-6) * w.double()
+    # the sum of squares of positive terms, a root, a quotient and two products: under 20 roundings of 2^-24
+    low, high = plain.between(h, h.abs() * 20 * 2.0 ** -24)
+    d = None if delta is None else delta.cuda()
+    other, r = torch.empty(rows, width, device="cuda"), junk_rows(rows, width)
+    ops().fp4_add_rmsnorm(stream.cuda(), d, w.cuda(), r, 1e-6, stream_out=other)
+    got, _ = plain.read(r.codes, r.scales, width)
+    assert torch.equal(other.cpu(), total)
+    assert bool(((got >= low) & (got <= high)).all())
+    assert pad_is_zero(r)
+    here, again = stream.cuda(), junk_rows(rows, width)
+    ops().fp4_add_rmsnorm(here, d, w.cuda(), again, 1e-6)
+    assert torch.equal(here, other) and torch.equal(again.codes, r.codes)
+
+
+# ---------------------------------------------------------------- products
+def product_tolerance(x, w):
+    """Per result: products of held values are exact, a float32 sum of K of them is off by at most the number of its roundings
+    times 2^-24 of the sum of their sizes; tensor cores add 64 at a time and may cut instead of round (2^-23)."""
+    return (x.abs() @ w.abs().t()) * ((x.shape[1] + 63) // 64 + 8) * 2.0 ** -23
+
+
+SIZES = [(1, 1, 1), (1, 8, 31), (1, 127, 32), (1, 130, 33), (2, 129, 64), (3, 64, 65), (7, 300, 127), (8, 128, 128), (9, 16, 129),
+         (16, 256, 256), (17, 257, 257), (33, 200, 300), (64, 520, 1000), (65, 100, 2008), (128, 384, 512), (129, 129, 640),
+         (200, 1111, 264), (300, 250, 4104), (512, 512, 1024), (700, 777, 776)]
+
+
+@pytest.mark.parametrize("out", list(DT))
+@pytest.mark.parametrize("rows,features,width", SIZES)
+def test_product(out, rows, features, width):
+    x, xv = held(normal(rows, width, rows + width))
+    w, wv = held(normal(features, width, features + 1, spread=False) * width ** -0.5)
+    y = torch.full((rows, features), 7.0, dtype=DT[out], device="cuda")
+    st = status()
+    ops().fp4_product(x, w, y, st)
+    assert int(st.item()) == 0
+    want, tol = xv @ wv.t(), product_tolerance(xv, wv)
+    if out == "bfloat16":
+        tol = tol + want.abs() * 2.0 ** -8
+    assert bool(((y.cpu().double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("out", list(DT))
+@pytest.mark.parametrize("rows", [1, 40, 300])
+@pytest.mark.parametrize("start,pitch", [(0, 320), (8, 336), (3, 301)])
+def test_product_into_columns(out, rows, start, pitch):
+    x, xv = held(normal(rows, 200, rows))
+    w, wv = held(normal(290, 200, 2, spread=False))
+    wide = torch.full((rows, pitch), 3.0, dtype=DT[out], device="cuda")
+    ops().fp4_product(x, w, wide[:, start:start + 290], status())
+    want = xv @ wv.t()
+    tol = product_tolerance(xv, wv) + (want.abs() * 2.0 ** -8 if out == "bfloat16" else 0)
+    assert bool(((wide[:, start:start + 290].cpu().double() - want).abs() <= tol).all())
+    assert bool((wide[:, :start] == 3).all()) and bool((wide[:, start + 290:] == 3).all())
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+def test_product_rows_beyond_the_first(rows):
+    """The first rows of a larger buffer whose other rows hold anything, their scales NaN."""
+    width, features = 520, 200
+    whole = junk_rows(rows + 150, width)
+    x = whole.first(rows)
+    data = normal(rows, width, 4)
+    ops().fp4_quantise(data.cuda(), x)
+    w, wv = held(normal(features, width, 8))
+    y = torch.empty(rows, features, device="cuda")
+    ops().fp4_product(x, w, y, status())
+    xv = plain.rounded(data.double())
+    assert bool(((y.cpu().double() - xv @ wv.t()).abs() <= product_tolerance(xv, wv)).all())
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+def test_product_of_what_is_not_finite(rows):
+    """A NaN scale reaches the results of its row of x or of w, and no others."""
+    xd, wd = normal(rows, 300, 1), normal(260, 300, 2)
+    xd[1, 77], wd[130, 299] = math.inf, math.nan
+    x, w = held(xd)[0], held(wd)[0]
+    y = torch.empty(rows, 260, device="cuda")
+    ops().fp4_product(x, w, y, status())
+    want = torch.zeros(rows, 260, dtype=torch.bool)
+    want[1], want[:, 130] = True, True
+    assert torch.equal(torch.isnan(y).cpu(), want)
+    assert bool(torch.isfinite(y.cpu()[~want]).all())
+
+
+def interleaved(gate, up):
+    i = gate.shape[0]
+    return torch.cat([gate.view(i // 8, 8, -1), up.view(i // 8, 8, -1)], dim=1).reshape(2 * i, -1)
+
+
+def gated_bounds(xv, wv, act):
+    """act(gate) * up in float64 and how far the kernel's may be from it: the products' own errors carried through (none of the
+    gates is steeper than 1.13), and 16 roundings of 2^-24 and the fast exponential's 2^-21 in the gate itself."""
+    both, tol = xv @ wv.t(), product_tolerance(xv, wv)
+    split = [t.view(t.shape[0], -1, 2, 8) for t in (both, tol)]
+    gate, up, dg, du = (t[:, :, k].reshape(t.shape[0], -1) for t in split for k in (0, 1))
+    if act == "silu":
+        f = gate * torch.sigmoid(gate)
+    elif act == "relu":
+        f = gate.clamp(min=0)
+    else:
+        f = 0.5 * gate * (1 + torch.tanh(math.sqrt(2 / math.pi) * (gate + 0.044715 * gate ** 3)))
+    a = f * up
+    # the gelu's 1 + tanh(y) loses what is below 2^-24 of 1, times the gate
+    lost = gate.abs() * up.abs() * 2.0 ** -22 if act == "gelu_tanh" else 0
+    return a, 1.13 * dg * (up.abs() + du) + f.abs() * du + a.abs() * 2.0 ** -19 + lost
+
+
+@pytest.mark.parametrize("act", ["silu", "relu", "gelu_tanh"])
+@pytest.mark.parametrize("rows,inner,width", [(1, 8, 32), (1, 64, 100), (3, 40, 264), (8, 136, 1024), (24, 200, 520), (33, 504, 256),
+                                              (130, 1000, 384), (300, 320, 600), (513, 600, 512)])
+def test_gated_product(act, rows, inner, width):
+    x, xv = held(normal(rows, width, rows))
+    w, wv = held(interleaved(normal(inner, width, 1, False), normal(inner, width, 2, False)) * width ** -0.5)
+    a, slack = gated_bounds(xv, wv, act)
+    low, high = plain.between(a, slack)
+    r = junk_rows(rows, inner)
+    st = status()
+    ops().fp4_gated_product(x, w, r, st, activation=act)
+    got, _ = plain.read(r.codes, r.scales, inner)
+    assert int(st.item()) == 0
+    assert bool(((got >= low) & (got <= high)).all())
+    assert pad_is_zero(r)
+
+
+@pytest.mark.parametrize("rows", [2, 260])
+def test_gated_product_of_what_is_not_finite(rows):
+    xd = normal(rows, 128, 1)
+    xd[1, 5] = math.nan
+    x = held(xd)[0]
+    w = held(interleaved(normal(72, 128, 1, False), normal(72, 128, 2, False)))[0]
+    r = junk_rows(rows, 72)
+    ops().fp4_gated_product(x, w, r, status())
+    got, byte = plain.read(r.codes, r.scales, 72)
+    assert bool((byte[1] == 255).all())
+    assert bool(torch.isfinite(got[0]).all()) and bool((byte[0] < 255).all())
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("rows,width,inner", [(1, 256, 520), (24, 512, 1000), (300, 264, 328)])
+def test_feed_forward_is_its_parts(dtype, rows, width, inner):
+    o = ops()
+    stream, delta = normal(rows, width, 1).cuda(), (normal(rows, width, 2) * 0.3).to(DT[dtype]).cuda()
+    norm = (1 + 0.1 * normal(1, width, 3, False)[0]).cuda()
+    gu = held(interleaved(normal(inner, width, 4, False), normal(inner, width, 5, False)) * width ** -0.5)[0]
+    down = held(normal(width, inner, 6, False) * inner ** -0.5)[0]
+    h, a = o.fp4_rows(rows, width, "cuda"), o.fp4_rows(rows, inner, "cuda")
+    y, s, st = torch.empty(rows, width, dtype=DT[dtype], device="cuda"), torch.empty_like(stream), status()
+    o.fp4_feed_forward(stream, delta, norm, 1e-6, gu, down, h, a, y, st, stream_out=s)
+    h2, a2, y2, s2 = o.fp4_rows(rows, width, "cuda"), o.fp4_rows(rows, inner, "cuda"), torch.empty_like(y), torch.empty_like(stream)
+    o.fp4_add_rmsnorm(stream, delta, norm, h2, 1e-6, stream_out=s2)
+    o.fp4_gated_product(h2, gu, a2, st)
+    o.fp4_product(a2, down, y2, st)
+    assert int(st.item()) == 0
+    assert torch.equal(s, s2) and torch.equal(h.codes, h2.codes) and torch.equal(a.codes, a2.codes) and torch.equal(y, y2)
+    # and against 64 bits: as the last product of what the gate left
+    want = plain.read(a.codes, a.scales, inner)[0] @ plain.read(down.codes, down.scales, inner)[0].t()
+    tol = product_tolerance(plain.read(a.codes, a.scales, inner)[0], plain.read(down.codes, down.scales, inner)[0])
+    assert bool(((y.cpu().double() - want).abs() <= tol + (want.abs() * 2.0 ** -8 if dtype == "bfloat16" else 0)).all())
+    o.fp4_feed_forward(stream, delta, norm, 1e-6, gu, down, h, a, y, st)  # the stream in place
+    assert torch.equal(stream, s) and torch.equal(y, y2)
+
+
+# ---------------------------------------------------------------- calls
+@pytest.mark.parametrize("rows", [4, 333])
+def test_the_same_inputs_give_the_same_bits_on_any_stream(rows):
+    x, w = held(normal(rows, 2000, 1))[0], held(normal(600, 2000, 2))[0]
+    first = torch.empty(rows, 600, device="cuda")
+    ops().fp4_product(x, w, first, status())
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    again = [torch.empty_like(first) for _ in range(4)]
+    with torch.cuda.stream(side):
+        for y in again:
+            ops().fp4_product(x, w, y, status())
+    side.synchronize()
+    assert all(torch.equal(first, y) for y in again)
+
+
+def test_no_rows_is_no_work():
+    o = ops()
+    empty, st = o.fp4_rows(0, 64, "cuda"), status()
+    o.fp4_quantise(torch.empty(0, 64, device="cuda"), empty)
+    o.fp4_product(empty, o.fp4_rows(32, 64, "cuda"), torch.empty(0, 32, device="cuda"), st)
+    o.fp4_gated_product(empty, o.fp4_rows(32, 64, "cuda"), o.fp4_rows(0, 16, "cuda"), st)
+    o.fp4_add_rmsnorm(torch.empty(0, 64, device="cuda"), None, torch.ones(64, device="cuda"), empty, 1e-6)
+
+
+def test_refusals():
+    o = ops()
+    x, w, y, st = o.fp4_rows(4, 64, "cuda"), o.fp4_rows(32, 64, "cuda"), torch.empty(4, 32, device="cuda"), status()
+    with pytest.raises(o.KernelError, match="expected"):
+        o.fp4_product(x, o.fp4_rows(32, 96, "cuda"), y, st)
+    with pytest.raises(o.KernelError, match="out"):
+        o.fp4_product(x, w, torch.empty(4, 31, device="cuda"), st)
+    with pytest.raises(o.KernelError, match="out"):
+        o.fp4_product(x, w, torch.empty(32, 4, device="cuda").t(), st)
+    with pytest.raises(o.KernelError, match="float32 or bfloat16"):
+        o.fp4_product(x, w, y.half(), st)
+    with pytest.raises(o.KernelError, match="codes"):
+        o.fp4_product(o.Fp4Rows(x.codes[:, :16].contiguous(), x.scales, 64), w, y, st)
+    with pytest.raises(o.KernelError, match="scales"):
+        o.fp4_product(x, o.Fp4Rows(torch.zeros(200, 32, dtype=torch.uint8, device="cuda"), w.scales, 64),
+                      torch.empty(4, 200, device="cuda"), st)
+    with pytest.raises(o.KernelError, match="contiguous"):
+        o.fp4_product(o.Fp4Rows(torch.zeros(4, 64, dtype=torch.uint8, device="cuda")[:, :32], x.scales, 64), w, y, st)
+    odd = torch.zeros(4 * 32 + 8, dtype=torch.uint8, device="cuda")[8:].view(4, 32)
+    with pytest.raises(o.KernelError, match="misaligned"):
+        o.fp4_product(o.Fp4Rows(odd, x.scales, 64), w, y, st)
+    with pytest.raises(o.KernelError, match="float32 or bfloat16"):
+        o.fp4_quantise(torch.zeros(4, 64, device="cuda", dtype=torch.float16), x)
+    with pytest.raises(o.KernelError, match="contiguous values"):
+        o.fp4_quantise(torch.zeros(64, 4, device="cuda").t(), x)
+    with pytest.raises(o.KernelError, match="values"):
+        o.fp4_quantise(torch.zeros(4, 64, device="cuda"), x, values=torch.zeros(4, 63, device="cuda"))
+    with pytest.raises(o.KernelError, match="gate"):
+        o.fp4_gated_product(x, w, o.fp4_rows(4, 16, "cuda"), st, activation="limited")
+    with pytest.raises(o.KernelSizeError):
+        o.fp4_gated_product(x, o.fp4_rows(36, 64, "cuda"), o.fp4_rows(4, 18, "cuda"), st)
+    with pytest.raises(o.KernelSizeError):
+        o.fp4_add_rmsnorm(torch.zeros(1, 32776, device="cuda"), None, torch.ones(32776, device="cuda"),
+                          o.fp4_rows(1, 32776, "cuda"), 1e-6)
+    with pytest.raises(o.KernelError, match="delta"):
+        o.fp4_add_rmsnorm(torch.zeros(4, 64, device="cuda"), torch.zeros(3, 64, device="cuda"), torch.ones(64, device="cuda"), x, 1e-6)
+    with pytest.raises(o.KernelSizeError):
+        o.fp4_rows(2, 0, "cuda")
+    assert int(st.item()) == 0
+
+
+@pytest.mark.parametrize("rows,features,width", [(3, 200, 3000), (300, 600, 1024)])
+def test_a_wait_that_runs_out_is_given_up_cleanly(rows, features, width):
+    o = ops()
+    x, xv = held(normal(rows, width, 1))
+    w, wv = held(normal(features, width, 2, False))
+    y, st = torch.empty(rows, features, device="cuda"), status()
+    try:
+        o.set_wait_test(limit=1 << 14, drop_copy=1)
+        o.fp4_product(x, w, y, st)
+        torch.cuda.synchronize()
+        word = int(st.item())
+    finally:
+        o.set_wait_test()
+    assert word & 16, f"status {word}: the time-out bit is not set"
+    st.zero_()
+    o.fp4_product(x, w, y, st)
+    assert int(st.item()) == 0
+    assert bool(((y.cpu().double() - xv @ wv.t()).abs() <= product_tolerance(xv, wv)).all())
