@@ -115,7 +115,7 @@ def _round_rows(x):
     byte = torch.where(top >= 0x7F800000, 255, (((top + 0x1FFFFF) >> 23) - 2).clamp(min=0))
     a = (x / _scale_of(byte)[..., None]).abs()
     code = ((a > 0.25).to(torch.uint8) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5))
-    code = code + 8 * (torch.signbit(x) & (byte != 255)[..., None])
+    code = code + 8 * (torch.signbit(x) & (byte != 255)[..., None]).to(torch.uint8)
     return code.view(r, blocks * BLOCK), byte.to(torch.uint8)
 
 
