@@ -106,6 +106,7 @@ static int fp4_quantise_launch(const void* x, long long x_pitch, uint8_t* codes,
   else
     q3::launch(fp4_quantise_kernel<T, false, V>, dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)x, x_pitch, codes, scales,
                (V*)values, values_vec, K, pieces, items);
+  note_stream_written();  // a product after it may take these rows as its w, which it reads ahead of its wait
   return launch_status();
 }
 
@@ -179,7 +180,7 @@ static int fp4_add_rmsnorm_launch(const float* in, const void* delta, const floa
   else if (g == 2) Q3_NORM(2);
   else Q3_NORM(4);
 #undef Q3_NORM
-  note_stream_written();
+  note_stream_written();  // the stream, and rows that a product might take as its w
   return launch_status();
 }
 

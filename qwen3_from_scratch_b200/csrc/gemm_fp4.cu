@@ -1,23 +1,26 @@
 // Products of matrices held in microscaled 4-bit floating point (fp4.cuh) on the fifth-generation tensor cores:
 // y[T, N] = x[T, K] * w[N, K]^T, tcgen05.mma kind::mxf4 with a scale per 32 values of k on both sides, float32 accumulators
-// in tensor memory.
+// in tensor memory.  The results are stored as bfloat16 or float32; or, for a w whose rows alternate gate/up in blocks of eight,
+// the gate is applied and each 32 results are rounded to the same format, so that the [T, 2 I] product never goes to memory.
 //
-// A block computes a tile of 128 rows of x by BN rows of w.  Three roles:
+// Both kernels have the same three roles:
 //   warp 0 (one thread)  brings the codes of 256 values of k at a time (128 bytes of each row) into shared memory by TMA
-//                        with the 128-byte swizzle, and their scales by bulk copies of whole 512-byte tiles;
-//   warp 1 (one thread)  copies each tile of scales into tensor memory (tcgen05.cp, which the instructions behind it in
-//                        the same thread wait for) and issues four instructions of k = 64 per stage;
-//   warps 2..5           read the accumulator, a thread per row of x, and store bfloat16 or float32; or, for a w whose rows
-//                        alternate gate/up in blocks of eight, apply the gate and round each 32 results to the same format.
-// The instruction reads a row's scales of k = 64 from two of the four bytes of a tensor-memory column; which two is in the
-// instruction descriptor.
+//                        with the 128-byte swizzle, and their scales in whole 512-byte tiles;
+//   warp 1 (one thread)  copies each tile of scales into tensor memory (tcgen05.cp, in order with the instructions of the
+//                        same thread before and behind it) and issues four instructions of k = 64 per stage;
+//   the other warps      the epilogue.
+// An instruction reads a row's scales of k = 64 from two of the four bytes of a tensor-memory column; which two is in its
+// descriptor.  Every wait on an mbarrier is bounded, as in gemm_tc.cu.
+//
+// gemm_fp4_few_kernel: 128 x 128 tiles and, where the tiles are fewer than the blocks that the SMs hold, several blocks per
+// tile that share out the range of k and add their sums up through each other's shared memory (a cluster).
+// gemm_fp4_pair_kernel: 256 x 256 tiles by pairs of CTAs, for many tokens.
 #include "fp4.cuh"
 #include "tc_common.cuh"
 
 namespace q3 {
 
 constexpr int F4_BM = 128;
-constexpr int F4_THREADS = 192;
 
 struct F4Args {
   const uint8_t* x_scales;
@@ -58,56 +61,131 @@ __device__ __forceinline__ void f4_bulk_load(void* dst, const void* src, uint32_
                : "memory");
 }
 
-template <int BN>
-struct F4Shape {
-  static constexpr int A_BYTES = F4_BM * 128, B_BYTES = BN * 128;
-  static constexpr int SA_BYTES = 2 * FP4_TILE_BYTES, SB_BYTES = (BN / FP4_TILE) * 2 * FP4_TILE_BYTES;
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;
-  static constexpr int STAGES = 6;
-  static constexpr int BAR_BYTES = 256;
-  static constexpr size_t SMEM_BYTES = (size_t)STAGES * STAGE_BYTES + BAR_BYTES;
-  static constexpr uint32_t SCALE_COL = BN;  // behind the accumulator
-  static constexpr uint32_t TMEM_COLS = 2 * BN;
-};
-static_assert(F4Shape<128>::STAGE_BYTES % 1024 == 0, "stages keep the swizzle's alignment");
+// Epilogues of a thread that holds neighbouring columns of one row.
+// 32 columns, as they are.
+template <int EPI>
+__device__ __forceinline__ void f4_store_row(const uint32_t (&v)[32], const F4Args& p, int row, int col) {
+  using OutT = typename std::conditional<EPI == 0, __nv_bfloat16, float>::type;
+  OutT* dst = (OutT*)p.out + (size_t)row * p.ldc + col;
+  if (col + 32 <= p.N && ((uintptr_t)dst & 15) == 0) {
+#pragma unroll
+    for (int j = 0; j < 32 * (int)sizeof(OutT) / 16; ++j) {
+      if (EPI == 0)
+        reinterpret_cast<uint4*>(dst)[j] = make_uint4(pack2(v[8 * j], v[8 * j + 1]), pack2(v[8 * j + 2], v[8 * j + 3]),
+                                                      pack2(v[8 * j + 4], v[8 * j + 5]), pack2(v[8 * j + 6], v[8 * j + 7]));
+      else
+        reinterpret_cast<uint4*>(dst)[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col + j < p.N) dst[j] = from_float<OutT>(__uint_as_float(v[j]));
+  }
+}
+// 128 columns, gate and up in blocks of eight: two blocks of 32 results, their codes and two scales.
+__device__ __forceinline__ void f4_gated_row(const uint32_t (&v)[4][32], const F4Args& p, int row, int col) {
+  const int inner = p.N / 2, blocks = (inner + FP4_BLOCK - 1) / FP4_BLOCK, out_across = fp4_tiles(inner);
+  uint8_t* word = p.out_scales + fp4_scale_word(row, col / 256, out_across);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int j = col / 64 + h;
+    float a[32];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int g = i / 8 * 16 + i % 8;
+      a[i] = gated_f(__uint_as_float(v[2 * h + g / 32][g % 32]), __uint_as_float(v[2 * h + (g + 8) / 32][(g + 8) % 32]), p.act, 0.f);
+      if (j * 32 + i >= inner) a[i] = 0.f;
+      top = max(top, __float_as_uint(a[i]) & 0x7fffffffu);
+    }
+    const uint32_t byte = fp4_scale_byte(top);
+    const float inv = fp4_inverse_scale(byte);
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float s8[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s8[i] = a[8 * q + i] * inv;
+      w[q] = byte == 255u ? 0u : fp4_pack8(s8);
+    }
+    if (j < blocks) *reinterpret_cast<uint4*>(p.out_codes + (size_t)row * fp4_pitch(inner) + j * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    word[j % 4] = (uint8_t)byte;
+    // the last columns also clear the scales behind the last block, up to the end of their word
+    if (col + 128 >= p.N && j % 4 < 2) word[j % 4 + 2] = 0;
+  }
+}
 
-template <int BN, int EPI>
-__global__ void __launch_bounds__(F4_THREADS)
-gemm_fp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
-                const __grid_constant__ F4Args p, int* status) {
-  using S = F4Shape<BN>;
+// ---------------------------------------------------------------- a few tokens: tiles of 128 x 128, k shared out
+constexpr int F4_FEW_THREADS = 192;
+constexpr int F4_BAR_BYTES = 256;
+constexpr int F4_FEW_MAX_STAGES = 8;
+constexpr int F4_FEW_MAX_SPLIT = 8;
+constexpr int F4_SUM_PITCH = 132;  // floats of a row of sums in shared memory: keeps rows off each other's banks
+constexpr int F4_FEW_COLS = 256;   // tensor memory: 128 columns of sums, 16 of scales, rounded up to a power of two
+
+struct F4FewShape {
+  int a_rows, stages, split;  // rows of x per tile (a multiple of 8), stages of the ring, blocks per tile
+  __host__ __device__ int a_bytes() const { return a_rows * 128; }
+  __host__ __device__ int stage_bytes() const { return a_bytes() + 128 * 128 + 4 * FP4_TILE_BYTES; }
+};
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t address) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address) : "memory");
+  return v;
+}
+
+// Only the first a_rows rows of an x tile are brought in; the instruction reads 128, the rest being whatever follows in shared
+// memory (every byte is two valid codes), into rows of the accumulator that are not looked at.
+template <int EPI>
+__global__ void __launch_bounds__(F4_FEW_THREADS)
+gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                    const __grid_constant__ F4Args p, const F4FewShape shape, const int early, int* status) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  unsigned char* tiles = smem_raw;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw + (size_t)S::STAGES * S::STAGE_BYTES);
-  uint64_t* empty = full + S::STAGES;
-  uint64_t* acc_full = empty + S::STAGES;
+  const int stages = shape.stages, stage_bytes = shape.stage_bytes(), split = shape.split;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw + (size_t)stages * stage_bytes);
+  uint64_t* empty = full + stages;
+  uint64_t* acc_full = empty + stages;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_full + 1);
   __shared__ int abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int across = fp4_tiles(p.K);          // tiles of scales along k
-  const int k_stages = (across + 1) / 2;
-  const int w_tiles = fp4_tiles(p.N);
-  const int m0 = blockIdx.y * F4_BM, n0 = blockIdx.x * BN;
+  const int rank = blockIdx.x % split, tile = blockIdx.x / split;
+  const int across = fp4_tiles(p.K), k_stages = (across + 1) / 2;
+  const int k0 = (int)((long long)k_stages * rank / split), k_count = (int)((long long)k_stages * (rank + 1) / split) - k0;
+  const int m0 = blockIdx.y * F4_BM, n0 = tile * 128;
   const bool aligned = (s_addr(smem_raw) & 1023u) == 0;
   if (!aligned && threadIdx.x == 0) atomicOr(status, Q3_STATUS_TIMEOUT);
 
+  const uint8_t* w_scales = p.w_scales + ((size_t)tile * across + 2 * k0) * FP4_TILE_BYTES;
+  auto scale_bytes = [&](int it) { return (uint32_t)min(2, across - 2 * (k0 + it)) * FP4_TILE_BYTES; };  // the last stage may have one tile
+  auto load_w = [&](int it, int s) {
+    unsigned char* b = smem_raw + (size_t)s * stage_bytes + shape.a_bytes();
+    const uint32_t sf = scale_bytes(it);
+    mbar_expect_tx(&full[s], shape.a_bytes() + 128 * 128 + 2 * sf);
+    tma_load_2d(b, &map_w, &full[s], (k0 + it) * 64, n0);
+    f4_bulk_load(b + 128 * 128 + 2 * FP4_TILE_BYTES, w_scales + (size_t)it * 2 * FP4_TILE_BYTES, sf, &full[s]);
+  };
+  int ahead = 0;  // thread 0: how many of its first stages have their part of w under way
   if (threadIdx.x == 0) {
     tma_prefetch_map(&map_x);
     tma_prefetch_map(&map_w);
     abort_flag = 0;
-    for (int s = 0; s < S::STAGES; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     mbar_init(acc_full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (early && aligned)  // the launch before this one did not write w: its part of the ring's first round goes out now
+      for (; ahead < min(stages, k_count); ++ahead) load_w(ahead, ahead);
   }
-  pdl_wait();
+  pdl_wait();  // x comes from the kernel before this one
   pdl_launch_dependents();
+  // Tensor memory is taken only after the wait: a block that holds some while it waits for the kernel before it could keep
+  // that kernel's own blocks from ever getting theirs.
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(tmem_holder)),
-                 "r"(S::TMEM_COLS)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(tmem_holder)), "r"(F4_FEW_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -116,52 +194,49 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_holder;
 
+  const int rows_here = min(F4_BM, p.T - m0);
+  float* const sums = reinterpret_cast<float*>(smem_raw);  // over the ring, once every instruction has read it
   if (warp == 0) {
     if (lane == 0 && aligned) {
+      const uint8_t* x_scales = p.x_scales + ((size_t)blockIdx.y * across + 2 * k0) * FP4_TILE_BYTES;
       int it = 0;
-      for (; it < k_stages; ++it) {
-        const int s = it % S::STAGES, use = it / S::STAGES;
-        if (use > 0 && !mbar_wait(&empty[s], (use & 1) ^ 1, &abort_flag)) {
-          abort_flag = 1;
-          atomicOr(status, Q3_STATUS_TIMEOUT);
-          break;
+      for (; it < k_count; ++it) {
+        const int s = it % stages, use = it / stages;
+        if (it >= ahead) {
+          if (use > 0 && !mbar_wait(&empty[s], (use & 1) ^ 1, &abort_flag)) {
+            abort_flag = 1;
+            atomicOr(status, Q3_STATUS_TIMEOUT);
+            break;
+          }
+          load_w(it, s);
         }
-        const uint32_t sf = (uint32_t)min(2, across - 2 * it) * FP4_TILE_BYTES;  // the last stage may have one tile
-        int w_here = 0;
-        for (int j = 0; j < BN / FP4_TILE; ++j) w_here += n0 / FP4_TILE + j < w_tiles;
-        unsigned char* a = tiles + (size_t)s * S::STAGE_BYTES;
-        unsigned char *b = a + S::A_BYTES, *sa = b + S::B_BYTES, *sb = sa + S::SA_BYTES;
-        mbar_expect_tx(&full[s], S::A_BYTES + S::B_BYTES + sf * (1 + w_here));
-        tma_load_2d(b, &map_w, &full[s], it * 64, n0);
-        for (int j = 0; j < w_here; ++j)
-          f4_bulk_load(sb + j * S::SA_BYTES, p.w_scales + ((size_t)(n0 / FP4_TILE + j) * across + 2 * it) * FP4_TILE_BYTES, sf, &full[s]);
-        f4_bulk_load(sa, p.x_scales + ((size_t)blockIdx.y * across + 2 * it) * FP4_TILE_BYTES, sf, &full[s]);
+        unsigned char* a = smem_raw + (size_t)s * stage_bytes;
+        f4_bulk_load(a + shape.a_bytes() + 128 * 128, x_scales + (size_t)it * 2 * FP4_TILE_BYTES, scale_bytes(it), &full[s]);
         if (it == tc_drop_copy) continue;  // tests of the give-up path only (see tc_common.cuh)
-        tma_load_2d(a, &map_x, &full[s], it * 64, m0);
+        tma_load_2d(a, &map_x, &full[s], (k0 + it) * 64, m0);
       }
-      finish_copies(full, it, S::STAGES, tc_drop_copy, status);
+      finish_copies(full, max(it, ahead), stages, tc_drop_copy, status);
     }
   } else if (warp == 1) {
     if (lane == 0 && aligned) {
       bool ok = true;
-      for (int it = 0; it < k_stages; ++it) {
-        const int s = it % S::STAGES, use = it / S::STAGES;
+      for (int it = 0; it < k_count; ++it) {
+        const int s = it % stages, use = it / stages;
         if (!mbar_wait(&full[s], use & 1, &abort_flag)) {
           ok = false;
           break;
         }
         tcgen05_fence_after();
-        const unsigned char* a = tiles + (size_t)s * S::STAGE_BYTES;
-        const unsigned char *b = a + S::A_BYTES, *sa = b + S::B_BYTES, *sb = sa + S::SA_BYTES;
+        const unsigned char* a = smem_raw + (size_t)s * stage_bytes;
+        const unsigned char *b = a + shape.a_bytes(), *sa = b + 128 * 128, *sb = sa + 2 * FP4_TILE_BYTES;
         const uint64_t a_desc = umma_desc_sw128(a), b_desc = umma_desc_sw128(b);
-        const int halves = min(2, across - 2 * it);
+        const int halves = min(2, across - 2 * (k0 + it));
         for (int h = 0; h < halves; ++h) {
-          const uint32_t ta = tmem + S::SCALE_COL + h * 4, tb = tmem + S::SCALE_COL + 8 + h * (BN / 32);
+          const uint32_t ta = tmem + 128 + h * 8, tb = ta + 4;
           f4_copy_scales(ta, f4_scale_desc(sa + h * FP4_TILE_BYTES));
-          for (int j = 0; j < BN / FP4_TILE; ++j)
-            f4_copy_scales(tb + 4 * j, f4_scale_desc(sb + j * S::SA_BYTES + h * FP4_TILE_BYTES));
-          f4_mma(tmem, a_desc + 4 * h, b_desc + 4 * h, f4_idesc(BN, 0), ta, tb, (it | h) != 0);
-          f4_mma(tmem, a_desc + 4 * h + 2, b_desc + 4 * h + 2, f4_idesc(BN, 2), ta, tb, 1);
+          f4_copy_scales(tb, f4_scale_desc(sb + h * FP4_TILE_BYTES));
+          f4_mma(tmem, a_desc + 4 * h, b_desc + 4 * h, f4_idesc(128, 0), ta, tb, (it | h) != 0);
+          f4_mma(tmem, a_desc + 4 * h + 2, b_desc + 4 * h + 2, f4_idesc(128, 2), ta, tb, 1);
         }
         umma_commit(&empty[s]);
       }
@@ -173,112 +248,414 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       }
     }
   } else if (aligned) {
-    const int quarter = warp & 3, row = m0 + quarter * 32 + lane;
+    const int quarter = warp & 3, row = quarter * 32 + lane;
     const bool ready = mbar_wait(acc_full, 0, &abort_flag);
     if (!__all_sync(0xffffffffu, ready)) {
       if (lane == 0) {
         abort_flag = 1;
         atomicOr(status, Q3_STATUS_TIMEOUT);
       }
-    } else {
+    } else if (quarter * 32 < rows_here) {
       tcgen05_fence_after();
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
-      if (EPI == 2) {
-        const int inner = p.N / 2, blocks = (inner + FP4_BLOCK - 1) / FP4_BLOCK, out_across = fp4_tiles(inner);
-        const int first = n0 / 64;
-        // the last tile also clears the scales behind the last block, up to the end of their tile
-        const int end = n0 + BN >= p.N ? out_across * 4 : first + BN / 64;
 #pragma unroll 1
-        for (int j = first; j < end; ++j) {
-          uint32_t byte = 0, w[4] = {0, 0, 0, 0};
-          if (j < blocks) {
-            uint32_t v[2][32];
-            tmem_ld_32(acc + (uint32_t)(j - first) * 64, v[0]);
-            tmem_ld_32(acc + (uint32_t)(j - first) * 64 + 32, v[1]);
-            tmem_wait_ld();
-            float a[32];
-            uint32_t top = 0;
+      for (int c0 = 0; c0 < 128; c0 += 32) {
+        uint32_t v[32];
+        tmem_ld_32(acc + (uint32_t)c0, v);
+        tmem_wait_ld();
+        if (row < rows_here)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int g = i / 8 * 16 + i % 8;
-              a[i] = gated_f(__uint_as_float(v[g / 32][g % 32]), __uint_as_float(v[(g + 8) / 32][(g + 8) % 32]), p.act, 0.f);
-              if (j * 32 + i >= inner) a[i] = 0.f;
-              top = max(top, __float_as_uint(a[i]) & 0x7fffffffu);
-            }
-            byte = fp4_scale_byte(top);
-            const float inv = fp4_inverse_scale(byte);
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(sums + row * F4_SUM_PITCH + c0 + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      }
+    }
+  }
+  tcgen05_fence_before();
+  // Every thread gets here, whatever was given up, so the cluster's barriers need no bound.
+  if (split > 1) cluster_sync_all();
+  else __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(F4_FEW_COLS) : "memory");
+  }
+
+  // A warp per row of the tile, four columns to a lane; the tile's rows are shared out over the cluster's warps.  The blocks'
+  // sums are added in the order of their ranges of k.
+  const int inner = p.N / 2, out_across = fp4_tiles(inner), blocks = (inner + FP4_BLOCK - 1) / FP4_BLOCK;
+  for (int r = rank * (F4_FEW_THREADS / 32) + warp; r < rows_here; r += split * (F4_FEW_THREADS / 32)) {
+    const uint32_t at = s_addr(sums + r * F4_SUM_PITCH + lane * 4);
+    float4 v;
+    if (split == 1) {
+      v = *reinterpret_cast<const float4*>(sums + r * F4_SUM_PITCH + lane * 4);
+    } else {
+      float4 part[F4_FEW_MAX_SPLIT];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float s8[8];
+      for (int q = 0; q < F4_FEW_MAX_SPLIT; ++q)
+        if (q < split) part[q] = ld_cluster_f4(cluster_addr(at, q));
+      v = part[0];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) s8[i] = a[8 * q + i] * inv;
-              w[q] = byte == 255u ? 0u : fp4_pack8(s8);
-            }
-          }
-          if (row < p.T) {
-            if (j < blocks) *reinterpret_cast<uint4*>(p.out_codes + (size_t)row * fp4_pitch(inner) + j * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-            p.out_scales[fp4_scale_word(row, j / 4, out_across) + j % 4] = (uint8_t)byte;
-          }
+      for (int q = 1; q < F4_FEW_MAX_SPLIT; ++q)
+        if (q < split) {
+          v.x += part[q].x;
+          v.y += part[q].y;
+          v.z += part[q].z;
+          v.w += part[q].w;
         }
+    }
+    const int row = m0 + r, col = n0 + lane * 4;
+    if (EPI == 2) {
+      // lanes 4 g, 4 g + 1 hold eight gate columns, lanes 4 g + 2, 4 g + 3 their up columns: 32 results per 16 lanes
+      const float up[4] = {__shfl_xor_sync(0xffffffffu, v.x, 2), __shfl_xor_sync(0xffffffffu, v.y, 2),
+                           __shfl_xor_sync(0xffffffffu, v.z, 2), __shfl_xor_sync(0xffffffffu, v.w, 2)};
+      const float gate[4] = {v.x, v.y, v.z, v.w};
+      const int block = n0 / 64 + (lane >> 4), first = block * 32 + ((lane & 15) >> 2) * 8 + (lane & 1) * 4;
+      float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!(lane & 2) && first + i < inner) a[i] = gated_f(gate[i], up[i], p.act, 0.f);
+        top = max(top, __float_as_uint(a[i]) & 0x7fffffffu);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const uint32_t byte = fp4_scale_byte(top);
+      const float inv = fp4_inverse_scale(byte);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] *= inv;
+      uint32_t c = byte == 255u ? 0u : fp4_pack8(a);
+      c |= __shfl_xor_sync(0xffffffffu, c, 1) << 16;
+      if ((lane & 3) == 0 && block < blocks)
+        *reinterpret_cast<uint32_t*>(p.out_codes + (size_t)row * fp4_pitch(inner) + block * 16 + (lane & 15)) = c;
+      if ((lane & 15) == 0) {
+        uint8_t* word = p.out_scales + fp4_scale_word(row, block / 4, out_across);
+        word[block % 4] = (uint8_t)byte;
+        // the last tile also clears the scales behind the last block, up to the end of their word
+        if (n0 + 128 >= p.N && block % 4 < 2) word[block % 4 + 2] = 0;
+      }
+    } else if (EPI == 0) {
+      __nv_bfloat16* dst = (__nv_bfloat16*)p.out + (size_t)row * p.ldc + col;
+      if (col + 4 <= p.N && ((uintptr_t)dst & 7) == 0) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(__float_as_uint(v.x), __float_as_uint(v.y)),
+                                                    pack2(__float_as_uint(v.z), __float_as_uint(v.w)));
       } else {
-#pragma unroll 1
-        for (int c0 = 0; c0 < BN; c0 += 32) {
-          if (n0 + c0 >= p.N) break;
-          uint32_t v[32];
-          tmem_ld_32(acc + (uint32_t)c0, v);
-          tmem_wait_ld();
-          if (row < p.T) {
-            using OutT = typename std::conditional<EPI == 0, __nv_bfloat16, float>::type;
-            OutT* dst = (OutT*)p.out + (size_t)row * p.ldc + n0 + c0;
-            if (n0 + c0 + 32 <= p.N && ((uintptr_t)dst & 15) == 0) {
+        const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-              for (int j = 0; j < 32 * (int)sizeof(OutT) / 16; ++j) {
-                if (EPI == 0)
-                  reinterpret_cast<uint4*>(dst)[j] = make_uint4(pack2(v[8 * j], v[8 * j + 1]), pack2(v[8 * j + 2], v[8 * j + 3]),
-                                                               pack2(v[8 * j + 4], v[8 * j + 5]), pack2(v[8 * j + 6], v[8 * j + 7]));
-                else
-                  reinterpret_cast<uint4*>(dst)[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-              }
-            } else {
+        for (int i = 0; i < 4; ++i)
+          if (col + i < p.N) dst[i] = __float2bfloat16_rn(f[i]);
+      }
+    } else {
+      float* dst = (float*)p.out + (size_t)row * p.ldc + col;
+      if (col + 4 <= p.N && ((uintptr_t)dst & 15) == 0) {
+        *reinterpret_cast<float4*>(dst) = v;
+      } else {
+        const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (n0 + c0 + j < p.N) dst[j] = from_float<OutT>(__uint_as_float(v[j]));
-            }
+        for (int i = 0; i < 4; ++i)
+          if (col + i < p.N) dst[i] = f[i];
+      }
+    }
+  }
+  if (split > 1) cluster_sync_all();  // no block leaves while another reads its sums
+}
+
+// ---------------------------------------------------------------- many tokens: 256 x 256 tiles by pairs of CTAs
+// The CTA of rank r holds rows 128 r .. of the x tile and of the w tile, rows 128 r .. of the accumulator, its own rows' scales
+// and all of the w tile's scales; the roles are those of gemm_tc_pair_kernel (gemm_tc.cu).  An accumulator of 256 columns and
+// 24 columns of scales leave no room for a second accumulator, so the epilogue's warps take their 128 columns of a row into
+// registers at once and hand the accumulator back before they work on them.
+struct F4Pair {
+  static constexpr int STAGES = 6;
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = 128 * 128, SA_BYTES = 2 * FP4_TILE_BYTES, SB_BYTES = 4 * FP4_TILE_BYTES;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;  // 35 KB
+  static constexpr size_t SMEM_BYTES = (size_t)STAGES * STAGE_BYTES + F4_BAR_BYTES;
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr uint32_t COLS = 512;
+  static constexpr int GROUP = 8;  // tiles of x that are walked through for one tile of w before the next one
+};
+
+__device__ __forceinline__ void f4_mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+      : "memory");
+}
+// Each CTA of the pair copies from its own shared memory, at this place, into its own tensor memory.
+__device__ __forceinline__ void f4_copy_scales_pair(uint32_t tmem, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+
+// Tile number `i` of a walk over m_tiles x n_tiles in which GROUP tiles of x stay in the second-level cache.
+__device__ __forceinline__ void f4_tile(int i, int m_tiles, int n_tiles, int* m, int* n) {
+  const int per = F4Pair::GROUP * n_tiles, g = i / per, first = g * F4Pair::GROUP;
+  const int high = min(F4Pair::GROUP, m_tiles - first), j = i - g * per;
+  *m = first + j % high;
+  *n = j / high;
+}
+
+template <int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F4Pair::THREADS)
+gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                     const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_ws,
+                     const __grid_constant__ F4Args p, int* status) {
+  using S = F4Pair;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw + (size_t)S::STAGES * S::STAGE_BYTES);  // used in rank 0
+  uint64_t* empty = full + S::STAGES;
+  uint64_t* acc_full = empty + S::STAGES;
+  uint64_t* acc_empty = acc_full + 1;  // used in rank 0
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 1);
+  __shared__ int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int across = fp4_tiles(p.K), k_stages = (across + 1) / 2;
+  const int m_tiles = (p.T + 255) / 256, n_tiles = (p.N + 255) / 256;
+  const bool aligned = (s_addr(smem_raw) & 1023u) == 0;  // the same in both CTAs
+  const int num_tiles = aligned ? m_tiles * n_tiles : 0;
+  if (!aligned && threadIdx.x == 0) atomicOr(status, Q3_STATUS_TIMEOUT);
+  auto give_up = [&]() {  // one thread
+    abort_flag = 1;
+    st_cluster_u32(cluster_addr(s_addr(&abort_flag), rank ^ 1u), 1u);
+    atomicOr(status, Q3_STATUS_TIMEOUT);
+  };
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_map(&map_x);
+    tma_prefetch_map(&map_w);
+    tma_prefetch_map(&map_xs);
+    tma_prefetch_map(&map_ws);
+    abort_flag = 0;
+    *tmem_holder = 0;
+    for (int s = 0; s < S::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 2 * S::EPI_WARPS);  // the epilogue warps of both CTAs
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  cluster_sync_all();
+  pdl_wait();  // x comes from the kernel before this one
+  pdl_launch_dependents();
+  if (warp == 1) {  // only after the wait, as above; the same warp of both CTAs asks, for the pair
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(tmem_holder)), "r"(S::COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_holder;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = pair; tile < num_tiles && ok; tile += pairs) {
+        int m, n;
+        f4_tile(tile, m_tiles, n_tiles, &m, &n);
+        for (int kt = 0; kt < k_stages; ++kt, ++it) {
+          const int s = it % S::STAGES;
+          const uint32_t use = it / S::STAGES;
+          if (use > 0 && !mbar_wait(&empty[s], (use & 1) ^ 1, &abort_flag)) {
+            give_up();
+            ok = false;
+            break;
           }
+          unsigned char* a = smem_raw + (size_t)s * S::STAGE_BYTES;
+          unsigned char *b = a + S::A_BYTES, *sa = b + S::B_BYTES, *sb = sa + S::SA_BYTES;
+          const uint32_t bar = cluster_addr(s_addr(&full[s]), 0);
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * S::STAGE_BYTES);
+          tma_load_2d_pair(b, &map_w, bar, kt * 64, n * 256 + (int)rank * 128);
+          tma_load_2d_pair(sb, &map_ws, bar, kt * 256, n * 2);
+          tma_load_2d_pair(sa, &map_xs, bar, kt * 256, m * 2 + (int)rank);
+          if ((int)it == tc_drop_copy && rank == 0) continue;  // tests of the give-up path only (see tc_common.cuh)
+          tma_load_2d_pair(a, &map_x, bar, kt * 64, m * 256 + (int)rank * 128);
         }
+      }
+      if (rank == 0) finish_copies(full, it, S::STAGES, tc_drop_copy, status);  // its barriers count both CTAs' copies
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      uint32_t it = 0, t = 0;
+      bool ok = true;
+      for (int tile = pair; tile < num_tiles && ok; tile += pairs, ++t) {
+        if (t > 0 && !mbar_wait_cluster(acc_empty, (t & 1) ^ 1, &abort_flag)) {
+          ok = false;
+          break;
+        }
+        tcgen05_fence_after();
+        for (int kt = 0; kt < k_stages; ++kt, ++it) {
+          const int s = it % S::STAGES;
+          if (!mbar_wait_cluster(&full[s], (it / S::STAGES) & 1, &abort_flag)) {
+            ok = false;
+            break;
+          }
+          tcgen05_fence_after();
+          const unsigned char* a = smem_raw + (size_t)s * S::STAGE_BYTES;
+          const unsigned char *b = a + S::A_BYTES, *sa = b + S::B_BYTES, *sb = sa + S::SA_BYTES;
+          const uint64_t a_desc = umma_desc_sw128(a), b_desc = umma_desc_sw128(b);
+          const int halves = min(2, across - 2 * kt);
+          for (int h = 0; h < halves; ++h) {
+            const uint32_t ta = tmem + 256 + h * 4, tb = tmem + 264 + h * 8;
+            f4_copy_scales_pair(ta, f4_scale_desc(sa + h * FP4_TILE_BYTES));
+            f4_copy_scales_pair(tb, f4_scale_desc(sb + h * FP4_TILE_BYTES));
+            f4_copy_scales_pair(tb + 4, f4_scale_desc(sb + S::SA_BYTES + h * FP4_TILE_BYTES));
+            f4_mma_pair(tmem, a_desc + 4 * h, b_desc + 4 * h, f4_idesc(256, 0, 256), ta, tb, (kt | h) != 0);
+            f4_mma_pair(tmem, a_desc + 4 * h + 2, b_desc + 4 * h + 2, f4_idesc(256, 2, 256), ta, tb, 1);
+          }
+          umma_commit_pair(&empty[s]);
+        }
+        if (ok) umma_commit_pair(acc_full);
+      }
+      if (!ok) give_up();
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t release = cluster_addr(s_addr(acc_empty), 0);
+    uint32_t t = 0;
+    for (int tile = pair; tile < num_tiles; tile += pairs, ++t) {
+      int m, n;
+      f4_tile(tile, m_tiles, n_tiles, &m, &n);
+      const bool ready = mbar_wait(acc_full, t & 1, &abort_flag);
+      if (!__all_sync(0xffffffffu, ready)) {
+        if (lane == 0) give_up();
+        break;
+      }
+      tcgen05_fence_after();
+      const int row = m * 256 + (int)rank * 128 + quarter * 32 + lane, n0 = n * 256 + half * 128;
+      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)half * 128;
+      uint32_t v[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32(acc + 32 * c, v[c]);
+      tmem_wait_ld();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(release);
+      if (row >= p.T || n0 >= p.N) continue;
+      if (EPI == 2) {
+        f4_gated_row(v, p, row, n0);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (n0 + 32 * c < p.N) f4_store_row<EPI>(v[c], p, row, n0 + 32 * c);
       }
     }
   }
   tcgen05_fence_before();
   __syncthreads();
-  if (warp == 1) {
-    __syncwarp();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM_COLS) : "memory");
+  cluster_sync_all();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
+}
+// A launch with blocks in clusters of `cluster` along x.
+template <typename... KArgs, typename... Args>
+static int f4_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl_enabled() && g_launch_early) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
   }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  g_plain_launch_stream.store((uintptr_t)stream, std::memory_order_relaxed);
+  return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+// The scales [tiles, across * 512 bytes] as boxes of 1,024 bytes x `rows` rows of tiles; beyond their end: zeros.
+static int f4_scale_map(CUtensorMap* map, const void* ptr, uint64_t tiles, uint64_t across, uint32_t rows) {
+  PFN_cuTensorMapEncodeTiled enc = tensor_map_encoder();
+  if (!enc) return Q3_ERR_DRIVER;
+  const cuuint64_t dims[2] = {across * (FP4_TILE_BYTES / 4), tiles};
+  const cuuint64_t strides[1] = {across * FP4_TILE_BYTES};
+  const cuuint32_t box[2] = {2 * FP4_TILE_BYTES / 4, rows};
+  const cuuint32_t elem[2] = {1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(ptr), dims, strides, box, elem,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : Q3_ERR_DRIVER;
 }
 
 template <int EPI>
-static int gemm_fp4_launch(const void* x_codes, const void* w_codes, const F4Args& p, int* status, cudaStream_t stream) {
-  constexpr int BN = 128;
-  using S = F4Shape<BN>;
+static int gemm_fp4_few_launch(const CUtensorMap& map_x, const CUtensorMap& map_w, const F4Args& p, const F4FewShape& shape, int early,
+                               int* status, cudaStream_t stream) {
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(gemm_fp4_kernel<BN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM_BYTES);
+    cudaError_t e = cudaFuncSetAttribute(gemm_fp4_few_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
     if (e != cudaSuccess) return (int)e;
     configured = true;
   }
-  const long long n_tiles = (p.N + BN - 1) / BN, m_tiles = (p.T + F4_BM - 1) / F4_BM;
-  if (n_tiles > 0x7fffffffLL || m_tiles > 65535) return Q3_ERR_SIZE;
+  const long long blocks = (long long)((p.N + 127) / 128) * shape.split, m_tiles = (p.T + F4_BM - 1) / F4_BM;
+  if (blocks > 0x7fffffffLL || m_tiles > 65535) return Q3_ERR_SIZE;
+  const int code = f4_launch(gemm_fp4_few_kernel<EPI>, dim3((unsigned)blocks, (unsigned)m_tiles), F4_FEW_THREADS,
+                             (size_t)shape.stages * shape.stage_bytes() + F4_BAR_BYTES, shape.split, stream, map_x, map_w, p, shape,
+                             early, status);
+  const int last = launch_status();
+  return code ? code : last;
+}
+
+template <int EPI>
+static int gemm_fp4_pair_launch(const CUtensorMap& map_x, const CUtensorMap& map_w, const F4Args& p, int* status, cudaStream_t stream) {
+  static bool configured = false;
+  if (!configured) {
+    cudaError_t e = cudaFuncSetAttribute(gemm_fp4_pair_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F4Pair::SMEM_BYTES);
+    if (e != cudaSuccess) return (int)e;
+    configured = true;
+  }
+  CUtensorMap map_xs, map_ws;
+  const uint64_t across = fp4_tiles(p.K);
+  int code = f4_scale_map(&map_xs, p.x_scales, fp4_tiles(p.T), across, 1);
+  if (code) return code;
+  code = f4_scale_map(&map_ws, p.w_scales, fp4_tiles(p.N), across, 2);
+  if (code) return code;
+  const long long tiles = (long long)((p.N + 255) / 256) * ((p.T + 255) / 256);
+  if (tiles > 0x3fffffffLL) return Q3_ERR_SIZE;
+  const long long slots = sm_count() / 2;
+  code = f4_launch(gemm_fp4_pair_kernel<EPI>, dim3((unsigned)(2 * (tiles < slots ? tiles : slots))), F4Pair::THREADS,
+                   F4Pair::SMEM_BYTES, 1, stream, map_x, map_w, map_xs, map_ws, p, status);
+  const int last = launch_status();
+  return code ? code : last;
+}
+
+// early: w was not written by the launch before this one.
+template <int EPI>
+static int gemm_fp4(const void* x_codes, const void* w_codes, const F4Args& p, int early, int* status, cudaStream_t stream) {
+  const int sms = sm_count();
+  const bool pair = p.T > 256 && (long long)((p.T + 255) / 256) * ((p.N + 255) / 256) >= sms / 4;
   // the maps take two bytes of codes as one bfloat16: only bytes move
   CUtensorMap map_x, map_w;
   const uint64_t cols = fp4_pitch(p.K) / 2;
-  int code = make_map(&map_x, x_codes, (uint64_t)p.T, cols, F4_BM);
+  F4FewShape shape{};
+  shape.a_rows = pair || p.T >= F4_BM ? F4_BM : (p.T + 7) / 8 * 8;
+  int code = make_map(&map_x, x_codes, (uint64_t)p.T, cols, shape.a_rows);
   if (code) return code;
-  code = make_map(&map_w, w_codes, (uint64_t)p.N, cols, BN);
+  code = make_map(&map_w, w_codes, (uint64_t)p.N, cols, 128);
   if (code) return code;
-  q3::launch(gemm_fp4_kernel<BN, EPI>, dim3((unsigned)n_tiles, (unsigned)m_tiles), dim3(F4_THREADS), S::SMEM_BYTES, stream, map_x,
-             map_w, p, status);
-  return launch_status();
+  if (pair) return gemm_fp4_pair_launch<EPI>(map_x, map_w, p, status, stream);
+  const int k_stages = (fp4_tiles(p.K) + 1) / 2;
+  const long long tiles = (long long)((p.N + 127) / 128) * ((p.T + F4_BM - 1) / F4_BM);
+  shape.split = 1;
+  while (shape.split < F4_FEW_MAX_SPLIT && tiles * shape.split * 2 <= 2 * sms && shape.split * 4 <= k_stages) shape.split *= 2;
+  const int need = (k_stages + shape.split - 1) / shape.split, room = 110 * 1024 / shape.stage_bytes();
+  const int sums = (min(F4_BM, p.T) * F4_SUM_PITCH * 4 + shape.stage_bytes() - 1) / shape.stage_bytes();  // stages that the sums take
+  shape.stages = max(min(min(need, room), F4_FEW_MAX_STAGES), max(sums, 2));
+  return gemm_fp4_few_launch<EPI>(map_x, map_w, p, shape, early, status, stream);
 }
 
 static bool f4_sizes_ok(int T, int N, int K) { return N > 0 && K > 0 && T > 0 && K <= (1 << 30) && N <= (1 << 30); }
@@ -286,32 +663,46 @@ static bool f4_aligned(const void* a, const void* b, const void* c, const void* 
   return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) & 15) == 0;
 }
 
+static int fp4_product(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out, int T, int N,
+                       int K, long long ldc, int out_f32, int early, int* status, cudaStream_t stream) {
+  if (T <= 0) return 0;
+  if (!f4_sizes_ok(T, N, K) || ldc < N) return Q3_ERR_SIZE;
+  if (!f4_aligned(x_codes, x_scales, w_codes, w_scales)) return Q3_ERR_ALIGN;
+  const F4Args p{(const uint8_t*)x_scales, (const uint8_t*)w_scales, out, ldc, nullptr, nullptr, T, N, K, 0};
+  if (out_f32) return gemm_fp4<1>(x_codes, w_codes, p, early, status, stream);
+  return gemm_fp4<0>(x_codes, w_codes, p, early, status, stream);
+}
+
+static int fp4_gated_product(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out_codes,
+                             void* out_scales, int T, int N, int K, int act, int early, int* status, cudaStream_t stream) {
+  if (T <= 0) return 0;
+  if (!f4_sizes_ok(T, N, K) || N % 16 || (act != Q3_ACT_SILU && act != Q3_ACT_RELU && act != Q3_ACT_GELU_TANH)) return Q3_ERR_SIZE;
+  if (!f4_aligned(x_codes, x_scales, w_codes, w_scales) || !f4_aligned(out_codes, out_scales, nullptr, nullptr)) return Q3_ERR_ALIGN;
+  const F4Args p{(const uint8_t*)x_scales, (const uint8_t*)w_scales, nullptr, 0, (uint8_t*)out_codes, (uint8_t*)out_scales, T, N, K, act};
+  return gemm_fp4<2>(x_codes, w_codes, p, early, status, stream);
+}
+
 }  // namespace q3
+
+extern "C" int q3_fp4_add_rmsnorm(const float* in, const void* delta, int dtype, const float* w, float* out, void* codes,
+                                  void* scales, int R, int H, float eps, cudaStream_t stream);
 
 // out[T, N] (row pitch ldc) = x w^T of rows held in four bits; out_f32: float32 results, else bfloat16.
 extern "C" int q3_fp4_product(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out, int T,
                               int N, int K, long long ldc, int out_f32, int* status, cudaStream_t stream) {
-  if (T <= 0) return 0;
-  if (!q3::f4_sizes_ok(T, N, K) || ldc < N) return Q3_ERR_SIZE;
-  if (!q3::f4_aligned(x_codes, x_scales, w_codes, w_scales)) return Q3_ERR_ALIGN;
-  q3::F4Args p{(const uint8_t*)x_scales, (const uint8_t*)w_scales, out, ldc, nullptr, nullptr, T, N, K, 0};
-  if (out_f32) return q3::gemm_fp4_launch<1>(x_codes, w_codes, p, status, stream);
-  return q3::gemm_fp4_launch<0>(x_codes, w_codes, p, status, stream);
+  return q3::fp4_product(x_codes, x_scales, w_codes, w_scales, out, T, N, K, ldc, out_f32, q3::last_launch_was_plain(stream), status,
+                         stream);
 }
 
 // act(gate) * up as rows held in four bits: w's N = 2 I rows alternate gate/up in blocks of eight, the output has T rows of I.
 extern "C" int q3_fp4_gated_product(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales,
                                     void* out_codes, void* out_scales, int T, int N, int K, int act, int* status,
                                     cudaStream_t stream) {
-  if (T <= 0) return 0;
-  if (!q3::f4_sizes_ok(T, N, K) || N % 16 || (act != Q3_ACT_SILU && act != Q3_ACT_RELU && act != Q3_ACT_GELU_TANH)) return Q3_ERR_SIZE;
-  if (!q3::f4_aligned(x_codes, x_scales, w_codes, w_scales) || !q3::f4_aligned(out_codes, out_scales, nullptr, nullptr)) return Q3_ERR_ALIGN;
-  q3::F4Args p{(const uint8_t*)x_scales, (const uint8_t*)w_scales, nullptr, 0, (uint8_t*)out_codes, (uint8_t*)out_scales, T, N, K, act};
-  return q3::gemm_fp4_launch<2>(x_codes, w_codes, p, status, stream);
+  const int code = q3::fp4_gated_product(x_codes, x_scales, w_codes, w_scales, out_codes, out_scales, T, N, K, act,
+                                         q3::last_launch_was_plain(stream), status, stream);
+  q3::note_stream_written();  // rows that a product after it might take as its w
+  return code;
 }
-
-extern "C" int q3_fp4_add_rmsnorm(const float* in, const void* delta, int dtype, const float* w, float* out, void* codes,
-                                  void* scales, int R, int H, float eps, cudaStream_t stream);
 
 // A gated feed-forward behind its norm, in three launches: the norm's rows into h, the gated product into a, y = a w_down^T.
 extern "C" int q3_fp4_feed_forward(const float* stream_in, const void* delta, const float* norm, float* stream_out, float eps,
@@ -320,9 +711,10 @@ extern "C" int q3_fp4_feed_forward(const float* stream_in, const void* delta, co
                                    int H, int I, int act, int* status, cudaStream_t stream) {
   int code = q3_fp4_add_rmsnorm(stream_in, delta, dtype, norm, stream_out, h_codes, h_scales, T, H, eps, stream);
   if (code) return code;
-  code = q3_fp4_gated_product(h_codes, h_scales, gu_codes, gu_scales, a_codes, a_scales, T, 2 * I, H, act, status, stream);
+  // neither product's w was written by the launch before it, which is the one above it here
+  code = q3::fp4_gated_product(h_codes, h_scales, gu_codes, gu_scales, a_codes, a_scales, T, 2 * I, H, act, 1, status, stream);
   if (code) return code;
-  return q3_fp4_product(a_codes, a_scales, down_codes, down_scales, y, T, H, I, H, dtype == Q3_F32, status, stream);
+  return q3::fp4_product(a_codes, a_scales, down_codes, down_scales, y, T, H, I, H, dtype == Q3_F32, 1, status, stream);
 }
 
 // For the tests of the give-up path: see set_wait_test in tc_common.cuh.

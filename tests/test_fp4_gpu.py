@@ -153,7 +153,8 @@ def product_tolerance(x, w):
 
 SIZES = [(1, 1, 1), (1, 8, 31), (1, 127, 32), (1, 130, 33), (2, 129, 64), (3, 64, 65), (7, 300, 127), (8, 128, 128), (9, 16, 129),
          (16, 256, 256), (17, 257, 257), (33, 200, 300), (64, 520, 1000), (65, 100, 2008), (128, 384, 512), (129, 129, 640),
-         (200, 1111, 264), (300, 250, 4104), (512, 512, 1024), (700, 777, 776)]
+         (200, 1111, 264), (300, 250, 4104), (512, 512, 1024), (700, 777, 776),
+         (257, 4900, 160), (600, 3333, 776), (1030, 2200, 300)]  # the last three by pairs of CTAs
 
 
 @pytest.mark.parametrize("out", list(DT))
@@ -172,23 +173,24 @@ def test_product(out, rows, features, width):
 
 
 @pytest.mark.parametrize("out", list(DT))
-@pytest.mark.parametrize("rows", [1, 40, 300])
-@pytest.mark.parametrize("start,pitch", [(0, 320), (8, 336), (3, 301)])
-def test_product_into_columns(out, rows, start, pitch):
+@pytest.mark.parametrize("rows,features", [(1, 290), (40, 290), (300, 290), (520, 3790)])
+@pytest.mark.parametrize("start,more", [(0, 30), (8, 46), (3, 11)])
+def test_product_into_columns(out, rows, features, start, more):
     x, xv = held(normal(rows, 200, rows))
-    w, wv = held(normal(290, 200, 2, spread=False))
-    wide = torch.full((rows, pitch), 3.0, dtype=DT[out], device="cuda")
-    ops().fp4_product(x, w, wide[:, start:start + 290], status())
+    w, wv = held(normal(features, 200, 2, spread=False))
+    end = start + features
+    wide = torch.full((rows, features + more), 3.0, dtype=DT[out], device="cuda")
+    ops().fp4_product(x, w, wide[:, start:end], status())
     want = xv @ wv.t()
     tol = product_tolerance(xv, wv) + (want.abs() * 2.0 ** -8 if out == "bfloat16" else 0)
-    assert bool(((wide[:, start:start + 290].cpu().double() - want).abs() <= tol).all())
-    assert bool((wide[:, :start] == 3).all()) and bool((wide[:, start + 290:] == 3).all())
+    assert bool(((wide[:, start:end].cpu().double() - want).abs() <= tol).all())
+    assert bool((wide[:, :start] == 3).all()) and bool((wide[:, end:] == 3).all())
 
 
-@pytest.mark.parametrize("rows", [5, 300])
-def test_product_rows_beyond_the_first(rows):
+@pytest.mark.parametrize("rows,features", [(5, 200), (300, 200), (300, 5000)])
+def test_product_rows_beyond_the_first(rows, features):
     """The first rows of a larger buffer whose other rows hold anything, their scales NaN."""
-    width, features = 520, 200
+    width = 520
     whole = junk_rows(rows + 150, width)
     x = whole.first(rows)
     data = normal(rows, width, 4)
@@ -200,15 +202,15 @@ def test_product_rows_beyond_the_first(rows):
     assert bool(((y.cpu().double() - xv @ wv.t()).abs() <= product_tolerance(xv, wv)).all())
 
 
-@pytest.mark.parametrize("rows", [3, 200])
-def test_product_of_what_is_not_finite(rows):
+@pytest.mark.parametrize("rows,features", [(3, 260), (200, 260), (300, 4900)])
+def test_product_of_what_is_not_finite(rows, features):
     """A NaN scale reaches the results of its row of x or of w, and no others."""
-    xd, wd = normal(rows, 300, 1), normal(260, 300, 2)
+    xd, wd = normal(rows, 300, 1), normal(features, 300, 2)
     xd[1, 77], wd[130, 299] = math.inf, math.nan
     x, w = held(xd)[0], held(wd)[0]
-    y = torch.empty(rows, 260, device="cuda")
+    y = torch.empty(rows, features, device="cuda")
     ops().fp4_product(x, w, y, status())
-    want = torch.zeros(rows, 260, dtype=torch.bool)
+    want = torch.zeros(rows, features, dtype=torch.bool)
     want[1], want[:, 130] = True, True
     assert torch.equal(torch.isnan(y).cpu(), want)
     assert bool(torch.isfinite(y.cpu()[~want]).all())
@@ -239,7 +241,8 @@ def gated_bounds(xv, wv, act):
 
 @pytest.mark.parametrize("act", ["silu", "relu", "gelu_tanh"])
 @pytest.mark.parametrize("rows,inner,width", [(1, 8, 32), (1, 64, 100), (3, 40, 264), (8, 136, 1024), (24, 200, 520), (33, 504, 256),
-                                              (130, 1000, 384), (300, 320, 600), (513, 600, 512)])
+                                              (130, 1000, 384), (300, 320, 600), (513, 600, 512), (300, 2504, 136), (600, 1672, 264),
+                                              (520, 1736, 300)])
 def test_gated_product(act, rows, inner, width):
     x, xv = held(normal(rows, width, rows))
     w, wv = held(interleaved(normal(inner, width, 1, False), normal(inner, width, 2, False)) * width ** -0.5)
@@ -293,10 +296,10 @@ def test_feed_forward_is_its_parts(dtype, rows, width, inner):
 
 
 # ---------------------------------------------------------------- calls
-@pytest.mark.parametrize("rows", [4, 333])
-def test_the_same_inputs_give_the_same_bits_on_any_stream(rows):
-    x, w = held(normal(rows, 2000, 1))[0], held(normal(600, 2000, 2))[0]
-    first = torch.empty(rows, 600, device="cuda")
+@pytest.mark.parametrize("rows,features", [(4, 600), (333, 600), (333, 4800)])
+def test_the_same_inputs_give_the_same_bits_on_any_stream(rows, features):
+    x, w = held(normal(rows, 2000, 1))[0], held(normal(features, 2000, 2))[0]
+    first = torch.empty(rows, features, device="cuda")
     ops().fp4_product(x, w, first, status())
     torch.cuda.synchronize()
     side = torch.cuda.Stream()
@@ -306,6 +309,25 @@ def test_the_same_inputs_give_the_same_bits_on_any_stream(rows):
             ops().fp4_product(x, w, y, status())
     side.synchronize()
     assert all(torch.equal(first, y) for y in again)
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_a_product_right_behind_what_rounds_its_w(rows):
+    """The product reads w ahead of the kernel before it only where that kernel did not write it."""
+    o = ops()
+    x, xv = held(normal(rows, 4096, 1))
+    data = normal(5000, 4096, 2, False).cuda()
+    w, y, st = junk_rows(5000, 4096), torch.empty(rows, 5000, device="cuda"), status()
+    want = torch.empty_like(y)
+    o.fp4_quantise(data, w)
+    torch.cuda.synchronize()
+    o.fp4_product(x, w, want, st)
+    for _ in range(5):
+        w.codes.fill_(0xA5)
+        o.fp4_quantise(data, w)
+        o.fp4_product(x, w, y, st)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
 
 
 def test_no_rows_is_no_work():
@@ -358,7 +380,7 @@ def test_refusals():
     assert int(st.item()) == 0
 
 
-@pytest.mark.parametrize("rows,features,width", [(3, 200, 3000), (300, 600, 1024)])
+@pytest.mark.parametrize("rows,features,width", [(3, 200, 3000), (300, 600, 1024), (600, 3400, 1024)])
 def test_a_wait_that_runs_out_is_given_up_cleanly(rows, features, width):
     o = ops()
     x, xv = held(normal(rows, width, 1))
