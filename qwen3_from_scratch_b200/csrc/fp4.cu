@@ -119,6 +119,16 @@ fp4_add_rmsnorm_kernel(const float* stream_in, const T* __restrict__ delta, cons
                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int H, float eps,
                        bool vec) {
   __shared__ float scratch[32];
+  float wv[G][8];
+  auto load_weight = [&](int g) {
+    const int col = (g * blockDim.x + threadIdx.x) * 8;
+    if (vec) fp4_load_row8<float, true>(w, col, H, wv[g]);
+    else fp4_load_row8<float, false>(w, col, H, wv[g]);
+  };
+  constexpr bool AHEAD = G <= 2;  // no kernel writes the weight: it is read ahead of the wait where the registers suffice
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+    if (AHEAD) load_weight(g);
   pdl_wait();
   pdl_launch_dependents();
   const size_t r = blockIdx.x;
@@ -153,11 +163,9 @@ fp4_add_rmsnorm_kernel(const float* stream_in, const T* __restrict__ delta, cons
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     const int col = (g * blockDim.x + threadIdx.x) * 8;
-    float wv[8];
-    if (vec) fp4_load_row8<float, true>(w, col, H, wv);
-    else fp4_load_row8<float, false>(w, col, H, wv);
+    if (!AHEAD) load_weight(g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[g][i] = v[g][i] * rs * wv[i];
+    for (int i = 0; i < 8; ++i) v[g][i] = v[g][i] * rs * wv[g][i];
     uint32_t byte;
     const uint32_t c = fp4_round8(v[g], &byte);
     if (col < pitch * 2) *reinterpret_cast<uint32_t*>(codes + r * pitch + col / 2) = c;

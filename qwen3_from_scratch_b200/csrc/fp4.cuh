@@ -54,6 +54,11 @@ __device__ __forceinline__ uint32_t fp4_pack8(const float (&v)[8]) {
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
 }
+__device__ __forceinline__ uint32_t fp4_pack2(float lo, float hi) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tmov.b32 %0, {a, a, a, a};\n\t}" : "=r"(r) : "f"(lo), "f"(hi));
+  return r & 255u;
+}
 // What two codes (the low eight bits) stand for, before their scale.
 __device__ __forceinline__ float2 fp4_pair(uint32_t two) {
   uint32_t h;

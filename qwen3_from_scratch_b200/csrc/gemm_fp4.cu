@@ -4,9 +4,9 @@
 // the gate is applied and each 32 results are rounded to the same format, so that the [T, 2 I] product never goes to memory.
 //
 // Both kernels have the same three roles:
-//   warp 0 (one thread)  brings the codes of 256 values of k at a time (128 bytes of each row) into shared memory by TMA
+//   warp 0  brings the codes of 256 values of k at a time (128 bytes of each row) into shared memory by TMA
 //                        with the 128-byte swizzle, and their scales in whole 512-byte tiles;
-//   warp 1 (one thread)  copies each tile of scales into tensor memory (tcgen05.cp, in order with the instructions of the
+//   warp 1  copies each tile of scales into tensor memory (tcgen05.cp, in order with the instructions of the
 //                        same thread before and behind it) and issues four instructions of k = 64 per stage;
 //   the other warps      the epilogue.
 // An instruction reads a row's scales of k = 64 from two of the four bytes of a tensor-memory column; which two is in its
@@ -61,6 +61,38 @@ __device__ __forceinline__ void f4_bulk_load(void* dst, const void* src, uint32_
                : "memory");
 }
 
+// One lane of a converged warp, the same one every time.  The loader and the issuing role run their loops with the whole warp
+// and pick the lane only around the instructions: what those are given (descriptors, addresses) is then the same in all lanes
+// as the compiler sees it and stays in the uniform registers that the instructions want.  With the whole loop in one lane it is
+// moved there anew for every instruction: a stage of two 128-column halves took 985 clocks to issue instead of 522.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// A wait of a whole warp: true if every lane saw the phase complete.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+__device__ __forceinline__ bool warp_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity, abort_flag));
+}
+
+// a[i] = act(g[i]) * u[i].  SiLU and GELU's tanh form are g sigmoid(z): (1 + tanh(y)) / 2 = sigmoid(2 y).  The fast exponential and
+// division are off by a few times 2^-23, which moves a result across a boundary between two codes once in some 10^5 values; the
+// exact ones, one value after another, took 1.2 us of a call's last 1.9 where a lane has four values to do.
+template <int N>
+__device__ __forceinline__ void f4_gate(const float (&g)[N], const float (&u)[N], int act, float (&a)[N]) {
+  if (act == Q3_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = fmaxf(g[i], 0.f) * u[i];
+    return;
+  }
+  const float cubic = act == Q3_ACT_GELU_TANH ? 0.044715f : 0.f, slope = act == Q3_ACT_GELU_TANH ? 1.5957691216057308f : 1.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[i] = u[i] * __fdividef(g[i], 1.0f + __expf(-slope * g[i] * fmaf(cubic * g[i], g[i], 1.0f)));
+}
+
 // Epilogues of a thread that holds neighbouring columns of one row.
 // 32 columns, as they are.
 template <int EPI>
@@ -89,12 +121,17 @@ __device__ __forceinline__ void f4_gated_row(const uint32_t (&v)[4][32], const F
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int j = col / 64 + h;
-    float a[32];
+    float gate[32], up[32], a[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int c = i / 8 * 16 + i % 8;
+      gate[i] = __uint_as_float(v[2 * h + c / 32][c % 32]);
+      up[i] = __uint_as_float(v[2 * h + (c + 8) / 32][(c + 8) % 32]);
+    }
+    f4_gate<32>(gate, up, p.act, a);
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      const int g = i / 8 * 16 + i % 8;
-      a[i] = gated_f(__uint_as_float(v[2 * h + g / 32][g % 32]), __uint_as_float(v[2 * h + (g + 8) / 32][(g + 8) % 32]), p.act, 0.f);
       if (j * 32 + i >= inner) a[i] = 0.f;
       top = max(top, __float_as_uint(a[i]) & 0x7fffffffu);
     }
@@ -109,30 +146,52 @@ __device__ __forceinline__ void f4_gated_row(const uint32_t (&v)[4][32], const F
       w[q] = byte == 255u ? 0u : fp4_pack8(s8);
     }
     if (j < blocks) *reinterpret_cast<uint4*>(p.out_codes + (size_t)row * fp4_pitch(inner) + j * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-    word[j % 4] = (uint8_t)byte;
-    // the last columns also clear the scales behind the last block, up to the end of their word
-    if (col + 128 >= p.N && j % 4 < 2) word[j % 4 + 2] = 0;
+    word[j % 4] = (uint8_t)byte;  // beyond the last block: zero
+    if (col + 128 >= p.N && j % 4 < 2) word[j % 4 + 2] = 0;  // and so up to the end of the tile of scales
   }
 }
 
-// ---------------------------------------------------------------- a few tokens: tiles of 128 x 128, k shared out
+// ---------------------------------------------------------------- a few tokens: small tiles, k shared out
+// A tile is up to 128 rows of x by 64, 128 or 192 rows of w, and `split` blocks of a cluster share out its range of k.  What
+// bounds it is w's bytes where w is large and the chain of latencies between two kernels where it is not, so the sizes are chosen
+// (f4_few_shape) to give each SM one block that leaves room for a block of the next kernel, which then has its first stages of w
+// on their way while this one works.
+//
+// The blocks of a cluster send each row of sums, by asynchronous stores that the receiver's mbarrier counts, to the block that
+// finishes that row (rank r % split).  No block reads another's memory, so none has to stay for the others: a barrier of the
+// whole cluster behind the reading took 1.1 us, as long as a stage of the main loop takes three times over.
 constexpr int F4_FEW_THREADS = 192;
-constexpr int F4_BAR_BYTES = 256;
-constexpr int F4_FEW_MAX_STAGES = 8;
+constexpr int F4_BAR_BYTES = 512;
+constexpr int F4_FEW_MAX_STAGES = 24;
 constexpr int F4_FEW_MAX_SPLIT = 8;
-constexpr int F4_SUM_PITCH = 132;  // floats of a row of sums in shared memory: keeps rows off each other's banks
-constexpr int F4_FEW_COLS = 256;   // tensor memory: 128 columns of sums, 16 of scales, rounded up to a power of two
+constexpr int F4_FEW_COLS = 256;  // tensor memory: up to 192 columns of sums, two times 24 of scales
+constexpr int F4_FEW_SCALE_COLS = 24;
 
 struct F4FewShape {
-  int a_rows, stages, split;  // rows of x per tile (a multiple of 8), stages of the ring, blocks per tile
+  int a_rows, bn, stages, split;  // rows of x in a tile (a multiple of 8, at most 128), rows of w in it, stages of the ring, blocks
+  int depth;                      // stages that a block works through (the last one of a cluster may have fewer)
+  int split_inverse;              // 65536 / split, rounded up: (r * split_inverse) >> 16 = r / split for r < 128
+  int slots;                      // rows of sums that a block of the cluster receives from each (split > 1)
   __host__ __device__ int a_bytes() const { return a_rows * 128; }
-  __host__ __device__ int stage_bytes() const { return a_bytes() + 128 * 128 + 4 * FP4_TILE_BYTES; }
+  __host__ __device__ int b_bytes() const { return bn * 128; }
+  __host__ __device__ int w_scale_tiles() const { return (bn + FP4_TILE - 1) / FP4_TILE; }
+  __host__ __device__ int stage_bytes() const { return a_bytes() + b_bytes() + (1 + w_scale_tiles()) * 2 * FP4_TILE_BYTES; }
+  // the last stage's x tile is read as 128 rows
+  __host__ __device__ int ring_bytes() const { return stages * stage_bytes() + (128 * 128 > stage_bytes() ? 128 * 128 - stage_bytes() : 0); }
+  __host__ __device__ int received_bytes() const { return split > 1 ? split * slots * bn * 4 : 0; }
+  __host__ __device__ size_t smem_bytes() const { return (size_t)ring_bytes() + received_bytes() + F4_BAR_BYTES; }
 };
 
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t address) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address) : "memory");
-  return v;
+__device__ __forceinline__ uint32_t cluster_id() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
+  return r;
+}
+// Four values to `address` of the cluster's window; the mbarrier at `bar`, in the same block, counts their 16 bytes.
+__device__ __forceinline__ void st_async_v4(uint32_t address, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+               ::"r"(address), "r"(a), "r"(b), "r"(c), "r"(d), "r"(bar)
+               : "memory");
 }
 
 // Only the first a_rows rows of an x tile are brought in; the instruction reads 128, the rest being whatever follows in shared
@@ -140,33 +199,44 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t address) {
 template <int EPI>
 __global__ void __launch_bounds__(F4_FEW_THREADS)
 gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
-                    const __grid_constant__ F4Args p, const F4FewShape shape, const int early, int* status) {
+                    const __grid_constant__ F4Args p, const __grid_constant__ F4FewShape shape, const int early, int* status) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  const int stages = shape.stages, stage_bytes = shape.stage_bytes(), split = shape.split;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw + (size_t)stages * stage_bytes);
+  const int stages = shape.stages, stage_bytes = shape.stage_bytes(), split = shape.split, bn = shape.bn;
+  float* const received = reinterpret_cast<float*>(smem_raw + shape.ring_bytes());
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw + shape.ring_bytes() + shape.received_bytes());
   uint64_t* empty = full + stages;
   uint64_t* acc_full = empty + stages;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_full + 1);
+  uint64_t* sums_full = acc_full + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sums_full + 1);
   __shared__ int abort_flag;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = blockIdx.x % split, tile = blockIdx.x / split;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = split > 1 ? (int)cluster_rank() : 0, tile = split > 1 ? (int)cluster_id() : blockIdx.x;
   const int across = fp4_tiles(p.K), k_stages = (across + 1) / 2;
-  const int k0 = (int)((long long)k_stages * rank / split), k_count = (int)((long long)k_stages * (rank + 1) / split) - k0;
-  const int m0 = blockIdx.y * F4_BM, n0 = tile * 128;
+  const int k0 = rank * shape.depth, k_count = min(shape.depth, k_stages - k0);
+  const int m0 = blockIdx.y * F4_BM, n0 = tile * bn, rows_here = min(F4_BM, p.T - m0);
+  const int w_tile = n0 / FP4_TILE, w_here = min((n0 % FP4_TILE + bn + FP4_TILE - 1) / FP4_TILE, fp4_tiles(p.N) - w_tile);
   const bool aligned = (s_addr(smem_raw) & 1023u) == 0;
   if (!aligned && threadIdx.x == 0) atomicOr(status, Q3_STATUS_TIMEOUT);
 
-  const uint8_t* w_scales = p.w_scales + ((size_t)tile * across + 2 * k0) * FP4_TILE_BYTES;
   auto scale_bytes = [&](int it) { return (uint32_t)min(2, across - 2 * (k0 + it)) * FP4_TILE_BYTES; };  // the last stage may have one tile
   auto load_w = [&](int it, int s) {
     unsigned char* b = smem_raw + (size_t)s * stage_bytes + shape.a_bytes();
+    unsigned char* sb = b + shape.b_bytes() + 2 * FP4_TILE_BYTES;
     const uint32_t sf = scale_bytes(it);
-    mbar_expect_tx(&full[s], shape.a_bytes() + 128 * 128 + 2 * sf);
+    mbar_expect_tx(&full[s], shape.a_bytes() + shape.b_bytes() + (1 + w_here) * sf);
     tma_load_2d(b, &map_w, &full[s], (k0 + it) * 64, n0);
-    f4_bulk_load(b + 128 * 128 + 2 * FP4_TILE_BYTES, w_scales + (size_t)it * 2 * FP4_TILE_BYTES, sf, &full[s]);
+    for (int j = 0; j < w_here; ++j)
+      f4_bulk_load(sb + j * 2 * FP4_TILE_BYTES, p.w_scales + ((size_t)(w_tile + j) * across + 2 * (k0 + it)) * FP4_TILE_BYTES, sf, &full[s]);
   };
-  int ahead = 0;  // thread 0: how many of its first stages have their part of w under way
+  auto load_x = [&](int it, int s) {
+    unsigned char* a = smem_raw + (size_t)s * stage_bytes;
+    f4_bulk_load(a + shape.a_bytes() + shape.b_bytes(), p.x_scales + ((size_t)blockIdx.y * across + 2 * (k0 + it)) * FP4_TILE_BYTES,
+                 scale_bytes(it), &full[s]);
+    if (it != tc_drop_copy)  // tests of the give-up path only (see tc_common.cuh)
+      tma_load_2d(a, &map_x, &full[s], (k0 + it) * 64, m0);
+  };
+  int ahead = 0;  // thread 0: how many of its first stages are under way before the roles begin
   if (threadIdx.x == 0) {
     tma_prefetch_map(&map_x);
     tma_prefetch_map(&map_w);
@@ -176,12 +246,19 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       mbar_init(&empty[s], 1);
     }
     mbar_init(acc_full, 1);
+    mbar_init(sums_full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (early && aligned)  // the launch before this one did not write w: its part of the ring's first round goes out now
       for (; ahead < min(stages, k_count); ++ahead) load_w(ahead, ahead);
+    // the rows that this block finishes, from every block of the cluster
+    if (split > 1) mbar_expect_tx(sums_full, (uint32_t)(split * (((rows_here - rank + split - 1) * shape.split_inverse) >> 16) * bn * 4));
   }
+  __syncwarp();
+  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for before anything is sent
   pdl_wait();  // x comes from the kernel before this one
   pdl_launch_dependents();
+  if (threadIdx.x == 0)
+    for (int it = 0; it < ahead; ++it) load_x(it, it);
   // Tensor memory is taken only after the wait: a block that holds some while it waits for the kernel before it could keep
   // that kernel's own blocks from ever getting theirs.
   if (warp == 1) {
@@ -194,143 +271,171 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_holder;
 
-  const int rows_here = min(F4_BM, p.T - m0);
-  float* const sums = reinterpret_cast<float*>(smem_raw);  // over the ring, once every instruction has read it
   if (warp == 0) {
-    if (lane == 0 && aligned) {
-      const uint8_t* x_scales = p.x_scales + ((size_t)blockIdx.y * across + 2 * k0) * FP4_TILE_BYTES;
-      int it = 0;
-      for (; it < k_count; ++it) {
-        const int s = it % stages, use = it / stages;
-        if (it >= ahead) {
-          if (use > 0 && !mbar_wait(&empty[s], (use & 1) ^ 1, &abort_flag)) {
+    if (aligned) {
+      ahead = __shfl_sync(0xffffffffu, ahead, 0);
+      int it = ahead, s = ahead == stages ? 0 : ahead;
+      for (uint32_t parity = 1; it < k_count; ++it) {
+        if (it >= stages && !warp_wait(&empty[s], parity ^ 1, &abort_flag)) {
+          if (lane == 0) {
             abort_flag = 1;
             atomicOr(status, Q3_STATUS_TIMEOUT);
-            break;
           }
-          load_w(it, s);
+          break;
         }
-        unsigned char* a = smem_raw + (size_t)s * stage_bytes;
-        f4_bulk_load(a + shape.a_bytes() + 128 * 128, x_scales + (size_t)it * 2 * FP4_TILE_BYTES, scale_bytes(it), &full[s]);
-        if (it == tc_drop_copy) continue;  // tests of the give-up path only (see tc_common.cuh)
-        tma_load_2d(a, &map_x, &full[s], (k0 + it) * 64, m0);
+        if (elect_one()) {
+          load_w(it, s);
+          load_x(it, s);
+        }
+        __syncwarp();
+        if (++s == stages) {
+          s = 0;
+          if (it >= stages) parity ^= 1;
+        }
       }
-      finish_copies(full, max(it, ahead), stages, tc_drop_copy, status);
+      if (lane == 0) finish_copies(full, it, stages, tc_drop_copy, status);
+      __syncwarp();
     }
   } else if (warp == 1) {
-    if (lane == 0 && aligned) {
+    if (aligned) {
       bool ok = true;
-      for (int it = 0; it < k_count; ++it) {
-        const int s = it % stages, use = it / stages;
-        if (!mbar_wait(&full[s], use & 1, &abort_flag)) {
+      const uint32_t low = f4_idesc(bn, 0), high = f4_idesc(bn, 2);
+      uint32_t parity = 0;
+      for (int it = 0, s = 0; it < k_count; ++it) {
+        if (!warp_wait(&full[s], parity, &abort_flag)) {
           ok = false;
           break;
         }
         tcgen05_fence_after();
         const unsigned char* a = smem_raw + (size_t)s * stage_bytes;
-        const unsigned char *b = a + shape.a_bytes(), *sa = b + 128 * 128, *sb = sa + 2 * FP4_TILE_BYTES;
-        const uint64_t a_desc = umma_desc_sw128(a), b_desc = umma_desc_sw128(b);
-        const int halves = min(2, across - 2 * (k0 + it));
-        for (int h = 0; h < halves; ++h) {
-          const uint32_t ta = tmem + 128 + h * 8, tb = ta + 4;
-          f4_copy_scales(ta, f4_scale_desc(sa + h * FP4_TILE_BYTES));
-          f4_copy_scales(tb, f4_scale_desc(sb + h * FP4_TILE_BYTES));
-          f4_mma(tmem, a_desc + 4 * h, b_desc + 4 * h, f4_idesc(128, 0), ta, tb, (it | h) != 0);
-          f4_mma(tmem, a_desc + 4 * h + 2, b_desc + 4 * h + 2, f4_idesc(128, 2), ta, tb, 1);
+        const unsigned char *b = a + shape.a_bytes(), *sa = b + shape.b_bytes(), *sb = sa + 2 * FP4_TILE_BYTES;
+        const uint64_t a_desc = umma_desc_sw128(a), b_desc = umma_desc_sw128(b), sa_desc = f4_scale_desc(sa), sb_desc = f4_scale_desc(sb);
+        // the scales of this stage beside those of the last one, which its instructions may still read; a column per 32 rows
+        const uint32_t ta = tmem + bn + (it & 1) * F4_FEW_SCALE_COLS, tb = ta + 8, tb_here = tb + (n0 % FP4_TILE) / 32;
+        const bool both = across - 2 * (k0 + it) > 1;
+        if (elect_one()) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (h == 0 || both) {
+              f4_copy_scales(ta + 4 * h, sa_desc + h * (FP4_TILE_BYTES >> 4));
+              f4_copy_scales(tb + 8 * h, sb_desc + h * (FP4_TILE_BYTES >> 4));
+              if (w_here > 1) f4_copy_scales(tb + 8 * h + 4, sb_desc + (2 + h) * (FP4_TILE_BYTES >> 4));
+              f4_mma(tmem, a_desc + 4 * h, b_desc + 4 * h, low, ta + 4 * h, tb_here + 8 * h, (it | h) != 0);
+              f4_mma(tmem, a_desc + 4 * h + 2, b_desc + 4 * h + 2, high, ta + 4 * h, tb_here + 8 * h, 1);
+            }
+          umma_commit(&empty[s]);
+          if (it + 1 == k_count) umma_commit(acc_full);
         }
-        umma_commit(&empty[s]);
+        __syncwarp();
+        if (++s == stages) {
+          s = 0;
+          parity ^= 1;
+        }
       }
-      if (ok) {
-        umma_commit(acc_full);
-      } else {
+      if (!ok && lane == 0) {
         abort_flag = 1;
         atomicOr(status, Q3_STATUS_TIMEOUT);
       }
+      __syncwarp();
     }
-  } else if (aligned) {
+  }
+  // Every thread gets here, whatever was given up, so the cluster's barrier needs no bound.
+  if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  float* const sums = split > 1 ? received : reinterpret_cast<float*>(smem_raw);  // alone: over the ring, which nothing reads by then
+  if (warp >= 2 && aligned) {
     const int quarter = warp & 3, row = quarter * 32 + lane;
-    const bool ready = mbar_wait(acc_full, 0, &abort_flag);
-    if (!__all_sync(0xffffffffu, ready)) {
+    if (!warp_wait(acc_full, 0, &abort_flag)) {
       if (lane == 0) {
         abort_flag = 1;
         atomicOr(status, Q3_STATUS_TIMEOUT);
       }
+      __syncwarp();
     } else if (quarter * 32 < rows_here) {
       tcgen05_fence_after();
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
+      const int slot = (row * shape.split_inverse) >> 16, owner = row - slot * split;  // row / split, row % split
+      const uint32_t to = split > 1 ? cluster_addr(s_addr(received + (rank * shape.slots + slot) * bn), owner) : 0;
+      const uint32_t bar = split > 1 ? cluster_addr(s_addr(sums_full), owner) : 0;
 #pragma unroll 1
-      for (int c0 = 0; c0 < 128; c0 += 32) {
-        uint32_t v[32];
-        tmem_ld_32(acc + (uint32_t)c0, v);
+      for (int c0 = 0; c0 < bn; c0 += 64) {
+        uint32_t v[2][32];
+        tmem_ld_32(acc + (uint32_t)c0, v[0]);
+        tmem_ld_32(acc + (uint32_t)c0 + 32, v[1]);
         tmem_wait_ld();
-        if (row < rows_here)
+        if (row < rows_here) {
+          if (split > 1) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(sums + row * F4_SUM_PITCH + c0 + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            for (int j = 0; j < 16; ++j)
+              st_async_v4(to + (c0 + 4 * j) * 4, v[j / 8][4 * (j % 8)], v[j / 8][4 * (j % 8) + 1], v[j / 8][4 * (j % 8) + 2],
+                          v[j / 8][4 * (j % 8) + 3], bar);
+          } else {  // rows bn + 4 values apart, off each other's banks
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              *reinterpret_cast<uint4*>(sums + row * (bn + 4) + c0 + 4 * j) =
+                  make_uint4(v[j / 8][4 * (j % 8)], v[j / 8][4 * (j % 8) + 1], v[j / 8][4 * (j % 8) + 2], v[j / 8][4 * (j % 8) + 3]);
+          }
+        }
+        __syncwarp();
       }
     }
   }
   tcgen05_fence_before();
-  // Every thread gets here, whatever was given up, so the cluster's barriers need no bound.
-  if (split > 1) cluster_sync_all();
-  else __syncthreads();
+  __syncthreads();
   if (warp == 1) {
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(F4_FEW_COLS) : "memory");
   }
+  // A block that gave up does not cut this wait short: the others' sums may still be on their way into its memory.
+  int never = 0;
+  if (split > 1 && !warp_wait(sums_full, 0, &never)) {
+    if (lane == 0) atomicOr(status, Q3_STATUS_TIMEOUT);
+    return;
+  }
 
-  // A warp per row of the tile, four columns to a lane; the tile's rows are shared out over the cluster's warps.  The blocks'
-  // sums are added in the order of their ranges of k.
+  // Sixteen lanes finish 64 columns of a row, four to a lane.  The blocks' sums are added in the order of their ranges of k.
   const int inner = p.N / 2, out_across = fp4_tiles(inner), blocks = (inner + FP4_BLOCK - 1) / FP4_BLOCK;
-  for (int r = rank * (F4_FEW_THREADS / 32) + warp; r < rows_here; r += split * (F4_FEW_THREADS / 32)) {
-    const uint32_t at = s_addr(sums + r * F4_SUM_PITCH + lane * 4);
-    float4 v;
-    if (split == 1) {
-      v = *reinterpret_cast<const float4*>(sums + r * F4_SUM_PITCH + lane * 4);
-    } else {
-      float4 part[F4_FEW_MAX_SPLIT];
-#pragma unroll
-      for (int q = 0; q < F4_FEW_MAX_SPLIT; ++q)
-        if (q < split) part[q] = ld_cluster_f4(cluster_addr(at, q));
-      v = part[0];
-#pragma unroll
-      for (int q = 1; q < F4_FEW_MAX_SPLIT; ++q)
-        if (q < split) {
-          v.x += part[q].x;
-          v.y += part[q].y;
-          v.z += part[q].z;
-          v.w += part[q].w;
-        }
+  const int groups = bn / 64, my_rows = ((rows_here - rank + split - 1) * shape.split_inverse) >> 16;
+  const int items = my_rows * groups, l = lane & 15;
+  for (int i0 = warp * 2; i0 < items; i0 += 2 * (F4_FEW_THREADS / 32)) {
+    const int item = min(i0 + (lane >> 4), items - 1);  // lanes without an item of their own do the last one again
+    const int slot = groups == 1 ? item : groups == 2 ? item >> 1 : item / 3, g = item - slot * groups;
+    const float* mine = sums + slot * (split > 1 ? bn : bn + 4) + g * 64 + l * 4;
+    float4 v = *reinterpret_cast<const float4*>(mine);
+    for (int q = 1; q < split; ++q) {
+      const float4 u = *reinterpret_cast<const float4*>(mine + (size_t)q * shape.slots * bn);
+      v.x += u.x;
+      v.y += u.y;
+      v.z += u.z;
+      v.w += u.w;
     }
-    const int row = m0 + r, col = n0 + lane * 4;
+    const int row = m0 + (split > 1 ? slot * split + rank : slot), col = n0 + g * 64 + l * 4;
     if (EPI == 2) {
-      // lanes 4 g, 4 g + 1 hold eight gate columns, lanes 4 g + 2, 4 g + 3 their up columns: 32 results per 16 lanes
-      const float up[4] = {__shfl_xor_sync(0xffffffffu, v.x, 2), __shfl_xor_sync(0xffffffffu, v.y, 2),
-                           __shfl_xor_sync(0xffffffffu, v.z, 2), __shfl_xor_sync(0xffffffffu, v.w, 2)};
-      const float gate[4] = {v.x, v.y, v.z, v.w};
-      const int block = n0 / 64 + (lane >> 4), first = block * 32 + ((lane & 15) >> 2) * 8 + (lane & 1) * 4;
-      float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      uint32_t top = 0;
+      // Of four lanes two hold eight gate columns and two their up columns; each takes two of the eight results, the other
+      // operand from the lane two further.  Sixteen lanes have a block of 32.
+      const bool second = l & 2;
+      const float o0 = __shfl_xor_sync(0xffffffffu, second ? v.x : v.z, 2), o1 = __shfl_xor_sync(0xffffffffu, second ? v.y : v.w, 2);
+      const float gate[2] = {second ? o0 : v.x, second ? o1 : v.y}, up[2] = {second ? v.z : o0, second ? v.w : o1};
+      const int block = n0 / 64 + g, place = (l >> 2) * 4 + (l & 1) * 2 + (second ? 1 : 0);  // of the lane's two among the block's
+      float a[2];
+      f4_gate<2>(gate, up, p.act, a);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (!(lane & 2) && first + i < inner) a[i] = gated_f(gate[i], up[i], p.act, 0.f);
-        top = max(top, __float_as_uint(a[i]) & 0x7fffffffu);
-      }
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int i = 0; i < 2; ++i)
+        if (block * 32 + place * 2 + i >= inner) a[i] = 0.f;
+      const uint32_t half = lane < 16 ? 0xffffu : 0xffff0000u;
+      const uint32_t top = __reduce_max_sync(half, max(__float_as_uint(a[0]) & 0x7fffffffu, __float_as_uint(a[1]) & 0x7fffffffu));
       const uint32_t byte = fp4_scale_byte(top);
       const float inv = fp4_inverse_scale(byte);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] *= inv;
-      uint32_t c = byte == 255u ? 0u : fp4_pack8(a);
-      c |= __shfl_xor_sync(0xffffffffu, c, 1) << 16;
-      if ((lane & 3) == 0 && block < blocks)
-        *reinterpret_cast<uint32_t*>(p.out_codes + (size_t)row * fp4_pitch(inner) + block * 16 + (lane & 15)) = c;
-      if ((lane & 15) == 0) {
-        uint8_t* word = p.out_scales + fp4_scale_word(row, block / 4, out_across);
-        word[block % 4] = (uint8_t)byte;
-        // the last tile also clears the scales behind the last block, up to the end of their word
-        if (n0 + 128 >= p.N && block % 4 < 2) word[block % 4 + 2] = 0;
+      uint32_t c = byte == 255u ? 0u : fp4_pack2(a[0] * inv, a[1] * inv) << (8 * (place & 3));
+      c |= __shfl_xor_sync(0xffffffffu, c, 1);
+      c |= __shfl_xor_sync(0xffffffffu, c, 2);
+      if (block < blocks) {
+        if ((l & 3) == 0) *reinterpret_cast<uint32_t*>(p.out_codes + (size_t)row * fp4_pitch(inner) + block * 16 + l) = c;
+        if (l == 0) {
+          uint8_t* word = p.out_scales + fp4_scale_word(row, block / 4, out_across);
+          word[block % 4] = (uint8_t)byte;
+          if (block + 1 == blocks)  // and the scales behind the last block, up to the end of their tile, are zero
+            for (int j = block % 4 + 1; j < 4; ++j) word[j] = 0;
+        }
       }
     } else if (EPI == 0) {
       __nv_bfloat16* dst = (__nv_bfloat16*)p.out + (size_t)row * p.ldc + col;
@@ -355,7 +460,6 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       }
     }
   }
-  if (split > 1) cluster_sync_all();  // no block leaves while another reads its sums
 }
 
 // ---------------------------------------------------------------- many tokens: 256 x 256 tiles by pairs of CTAs
@@ -409,7 +513,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 1);
   __shared__ int abort_flag;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int across = fp4_tiles(p.K), k_stages = (across + 1) / 2;
@@ -453,67 +557,74 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
   const uint32_t tmem = *tmem_holder;
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (int tile = pair; tile < num_tiles && ok; tile += pairs) {
-        int m, n;
-        f4_tile(tile, m_tiles, n_tiles, &m, &n);
-        for (int kt = 0; kt < k_stages; ++kt, ++it) {
-          const int s = it % S::STAGES;
-          const uint32_t use = it / S::STAGES;
-          if (use > 0 && !mbar_wait(&empty[s], (use & 1) ^ 1, &abort_flag)) {
-            give_up();
-            ok = false;
-            break;
-          }
-          unsigned char* a = smem_raw + (size_t)s * S::STAGE_BYTES;
-          unsigned char *b = a + S::A_BYTES, *sa = b + S::B_BYTES, *sb = sa + S::SA_BYTES;
-          const uint32_t bar = cluster_addr(s_addr(&full[s]), 0);
+    uint32_t it = 0;
+    bool ok = true;
+    for (int tile = pair; tile < num_tiles && ok; tile += pairs) {
+      int m, n;
+      f4_tile(tile, m_tiles, n_tiles, &m, &n);
+      for (int kt = 0; kt < k_stages; ++kt, ++it) {
+        const int s = it % S::STAGES;
+        const uint32_t use = it / S::STAGES;
+        if (use > 0 && !warp_wait(&empty[s], (use & 1) ^ 1, &abort_flag)) {
+          if (lane == 0) give_up();
+          ok = false;
+          break;
+        }
+        unsigned char* a = smem_raw + (size_t)s * S::STAGE_BYTES;
+        unsigned char *b = a + S::A_BYTES, *sa = b + S::B_BYTES, *sb = sa + S::SA_BYTES;
+        const uint32_t bar = cluster_addr(s_addr(&full[s]), 0);
+        if (elect_one()) {
           if (rank == 0) mbar_expect_tx(&full[s], 2 * S::STAGE_BYTES);
           tma_load_2d_pair(b, &map_w, bar, kt * 64, n * 256 + (int)rank * 128);
           tma_load_2d_pair(sb, &map_ws, bar, kt * 256, n * 2);
           tma_load_2d_pair(sa, &map_xs, bar, kt * 256, m * 2 + (int)rank);
-          if ((int)it == tc_drop_copy && rank == 0) continue;  // tests of the give-up path only (see tc_common.cuh)
-          tma_load_2d_pair(a, &map_x, bar, kt * 64, m * 256 + (int)rank * 128);
+          if ((int)it != tc_drop_copy || rank != 0)  // tests of the give-up path only (see tc_common.cuh)
+            tma_load_2d_pair(a, &map_x, bar, kt * 64, m * 256 + (int)rank * 128);
         }
+        __syncwarp();
       }
-      if (rank == 0) finish_copies(full, it, S::STAGES, tc_drop_copy, status);  // its barriers count both CTAs' copies
     }
+    if (rank == 0 && lane == 0) finish_copies(full, it, S::STAGES, tc_drop_copy, status);  // its barriers count both CTAs' copies
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       uint32_t it = 0, t = 0;
       bool ok = true;
       for (int tile = pair; tile < num_tiles && ok; tile += pairs, ++t) {
-        if (t > 0 && !mbar_wait_cluster(acc_empty, (t & 1) ^ 1, &abort_flag)) {
+        if (t > 0 && !warp_wait_cluster(acc_empty, (t & 1) ^ 1, &abort_flag)) {
           ok = false;
           break;
         }
         tcgen05_fence_after();
         for (int kt = 0; kt < k_stages; ++kt, ++it) {
           const int s = it % S::STAGES;
-          if (!mbar_wait_cluster(&full[s], (it / S::STAGES) & 1, &abort_flag)) {
+          if (!warp_wait_cluster(&full[s], (it / S::STAGES) & 1, &abort_flag)) {
             ok = false;
             break;
           }
           tcgen05_fence_after();
           const unsigned char* a = smem_raw + (size_t)s * S::STAGE_BYTES;
           const unsigned char *b = a + S::A_BYTES, *sa = b + S::B_BYTES, *sb = sa + S::SA_BYTES;
-          const uint64_t a_desc = umma_desc_sw128(a), b_desc = umma_desc_sw128(b);
-          const int halves = min(2, across - 2 * kt);
-          for (int h = 0; h < halves; ++h) {
-            const uint32_t ta = tmem + 256 + h * 4, tb = tmem + 264 + h * 8;
-            f4_copy_scales_pair(ta, f4_scale_desc(sa + h * FP4_TILE_BYTES));
-            f4_copy_scales_pair(tb, f4_scale_desc(sb + h * FP4_TILE_BYTES));
-            f4_copy_scales_pair(tb + 4, f4_scale_desc(sb + S::SA_BYTES + h * FP4_TILE_BYTES));
-            f4_mma_pair(tmem, a_desc + 4 * h, b_desc + 4 * h, f4_idesc(256, 0, 256), ta, tb, (kt | h) != 0);
-            f4_mma_pair(tmem, a_desc + 4 * h + 2, b_desc + 4 * h + 2, f4_idesc(256, 2, 256), ta, tb, 1);
+          const uint64_t a_desc = umma_desc_sw128(a), b_desc = umma_desc_sw128(b), sa_desc = f4_scale_desc(sa), sb_desc = f4_scale_desc(sb);
+          // the scales of this stage beside those of the last one, which its instructions may still read
+          const uint32_t ta = tmem + 256 + (it & 1) * 24, tb = ta + 8;
+          const bool both = across - 2 * kt > 1;
+          if (elect_one()) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (h == 0 || both) {
+                f4_copy_scales_pair(ta + 4 * h, sa_desc + h * (FP4_TILE_BYTES >> 4));
+                f4_copy_scales_pair(tb + 8 * h, sb_desc + h * (FP4_TILE_BYTES >> 4));
+                f4_copy_scales_pair(tb + 8 * h + 4, sb_desc + (S::SA_BYTES >> 4) + h * (FP4_TILE_BYTES >> 4));
+                f4_mma_pair(tmem, a_desc + 4 * h, b_desc + 4 * h, f4_idesc(256, 0, 256), ta + 4 * h, tb + 8 * h, (kt | h) != 0);
+                f4_mma_pair(tmem, a_desc + 4 * h + 2, b_desc + 4 * h + 2, f4_idesc(256, 2, 256), ta + 4 * h, tb + 8 * h, 1);
+              }
+            umma_commit_pair(&empty[s]);
+            if (kt + 1 == k_stages) umma_commit_pair(acc_full);
           }
-          umma_commit_pair(&empty[s]);
+          __syncwarp();
         }
-        if (ok) umma_commit_pair(acc_full);
       }
-      if (!ok) give_up();
+      if (!ok && lane == 0) give_up();
     }
   } else {
     const int quarter = warp & 3, half = (warp - 2) >> 2;
@@ -597,17 +708,56 @@ static int gemm_fp4_few_launch(const CUtensorMap& map_x, const CUtensorMap& map_
                                int* status, cudaStream_t stream) {
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(gemm_fp4_few_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+    cudaError_t e = cudaFuncSetAttribute(gemm_fp4_few_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024);
+    if (e == cudaSuccess)  // a kernel that asks for less keeps its SM from taking a block of one that asks for more beside its own
+      e = cudaFuncSetAttribute(gemm_fp4_few_kernel<EPI>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return (int)e;
     configured = true;
   }
-  const long long blocks = (long long)((p.N + 127) / 128) * shape.split, m_tiles = (p.T + F4_BM - 1) / F4_BM;
+  const long long blocks = (long long)((p.N + shape.bn - 1) / shape.bn) * shape.split, m_tiles = (p.T + F4_BM - 1) / F4_BM;
   if (blocks > 0x7fffffffLL || m_tiles > 65535) return Q3_ERR_SIZE;
-  const int code = f4_launch(gemm_fp4_few_kernel<EPI>, dim3((unsigned)blocks, (unsigned)m_tiles), F4_FEW_THREADS,
-                             (size_t)shape.stages * shape.stage_bytes() + F4_BAR_BYTES, shape.split, stream, map_x, map_w, p, shape,
-                             early, status);
+  const int code = f4_launch(gemm_fp4_few_kernel<EPI>, dim3((unsigned)blocks, (unsigned)m_tiles), F4_FEW_THREADS, shape.smem_bytes(),
+                             shape.split, stream, map_x, map_w, p, shape, early, status);
   const int last = launch_status();
   return code ? code : last;
+}
+
+// The few-tokens kernel's tiles.  Blocks run one to an SM in rounds; a round takes its stages times what issuing one takes (clocks,
+// measured on one SM: 386, 415 and 470 for 64, 128 and 192 rows of w), and sharing out k costs the sending and adding of sums.
+static F4FewShape f4_few_shape(int T, int N, int K) {
+  F4FewShape best{};
+  double best_cost = 0;
+  const int sms = sm_count(), k_stages = (fp4_tiles(K) + 1) / 2, rows = T < F4_BM ? T : F4_BM;
+  for (int bn = 64; bn <= 192; bn += 64) {
+    const long long tiles = (long long)((N + bn - 1) / bn) * ((T + F4_BM - 1) / F4_BM);
+    for (int split = 1; split <= F4_FEW_MAX_SPLIT && split <= k_stages; ++split) {
+      const int depth = (k_stages + split - 1) / split;
+      if ((split - 1) * depth >= k_stages) continue;  // no block without a stage
+      const double rounds = (double)((tiles * split + sms - 1) / sms);
+      const double cost = rounds * (depth * (bn == 64 ? 386 : bn == 128 ? 415 : 470) + (split > 1 ? 600 + rows * bn / 2 : 0));
+      if (best.bn == 0 || cost < best_cost) {
+        best_cost = cost;
+        best.bn = bn;
+        best.split = split;
+        best.depth = depth;
+      }
+    }
+  }
+  best.a_rows = (rows + 7) / 8 * 8;
+  best.slots = (rows + best.split - 1) / best.split;
+  best.split_inverse = (65536 + best.split - 1) / best.split;
+  const int need = best.depth;
+  const int alone = best.split > 1 ? 0 : rows * (best.bn + 4) * 4;  // the sums' place over the ring
+  // half of an SM's shared memory, so that a block of the next kernel fits beside; all of it where that leaves under three stages
+  for (int room = 112 * 1024;; room = 224 * 1024) {
+    best.stages = (room - best.received_bytes() - F4_BAR_BYTES) / best.stage_bytes();
+    if (best.stages > need) best.stages = need;
+    if (best.stages > F4_FEW_MAX_STAGES) best.stages = F4_FEW_MAX_STAGES;
+    if (best.stages < 1) best.stages = 1;
+    if (room > 112 * 1024 || ((best.stages >= 3 || best.stages == need) && best.ring_bytes() >= alone)) break;
+  }
+  while (best.ring_bytes() < alone) ++best.stages;
+  return best;
 }
 
 template <int EPI>
@@ -615,6 +765,8 @@ static int gemm_fp4_pair_launch(const CUtensorMap& map_x, const CUtensorMap& map
   static bool configured = false;
   if (!configured) {
     cudaError_t e = cudaFuncSetAttribute(gemm_fp4_pair_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F4Pair::SMEM_BYTES);
+    if (e == cudaSuccess)  // a kernel that asks for less keeps its SM from taking a block of one that asks for more beside its own
+      e = cudaFuncSetAttribute(gemm_fp4_pair_kernel<EPI>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return (int)e;
     configured = true;
   }
@@ -638,23 +790,16 @@ template <int EPI>
 static int gemm_fp4(const void* x_codes, const void* w_codes, const F4Args& p, int early, int* status, cudaStream_t stream) {
   const int sms = sm_count();
   const bool pair = p.T > 256 && (long long)((p.T + 255) / 256) * ((p.N + 255) / 256) >= sms / 4;
+  F4FewShape shape{};
+  if (!pair) shape = f4_few_shape(p.T, p.N, p.K);
   // the maps take two bytes of codes as one bfloat16: only bytes move
   CUtensorMap map_x, map_w;
   const uint64_t cols = fp4_pitch(p.K) / 2;
-  F4FewShape shape{};
-  shape.a_rows = pair || p.T >= F4_BM ? F4_BM : (p.T + 7) / 8 * 8;
-  int code = make_map(&map_x, x_codes, (uint64_t)p.T, cols, shape.a_rows);
+  int code = cached_map(&map_x, x_codes, (uint64_t)p.T, cols, pair ? 128 : shape.a_rows);
   if (code) return code;
-  code = make_map(&map_w, w_codes, (uint64_t)p.N, cols, 128);
+  code = cached_map(&map_w, w_codes, (uint64_t)p.N, cols, pair ? 128 : shape.bn);
   if (code) return code;
   if (pair) return gemm_fp4_pair_launch<EPI>(map_x, map_w, p, status, stream);
-  const int k_stages = (fp4_tiles(p.K) + 1) / 2;
-  const long long tiles = (long long)((p.N + 127) / 128) * ((p.T + F4_BM - 1) / F4_BM);
-  shape.split = 1;
-  while (shape.split < F4_FEW_MAX_SPLIT && tiles * shape.split * 2 <= 2 * sms && shape.split * 4 <= k_stages) shape.split *= 2;
-  const int need = (k_stages + shape.split - 1) / shape.split, room = 110 * 1024 / shape.stage_bytes();
-  const int sums = (min(F4_BM, p.T) * F4_SUM_PITCH * 4 + shape.stage_bytes() - 1) / shape.stage_bytes();  // stages that the sums take
-  shape.stages = max(min(min(need, room), F4_FEW_MAX_STAGES), max(sums, 2));
   return gemm_fp4_few_launch<EPI>(map_x, map_w, p, shape, early, status, stream);
 }
 
