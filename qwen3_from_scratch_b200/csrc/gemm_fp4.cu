@@ -93,62 +93,81 @@ __device__ __forceinline__ void f4_gate(const float (&g)[N], const float (&u)[N]
   for (int i = 0; i < N; ++i) a[i] = u[i] * __fdividef(g[i], 1.0f + __expf(-slope * g[i] * fmaf(cubic * g[i], g[i], 1.0f)));
 }
 
-// Epilogues of a thread that holds neighbouring columns of one row.
-// 32 columns, as they are.
+// 128 bytes of results (32 float32 or 64 bfloat16 columns from `col` on) of each of the warp's 32 rows, a row to a lane, by way of
+// 4 KB of shared memory: there the lanes change places, so that eight of them store the 128 bytes of a row side by side.  Storing
+// from the accumulator's own order, 16 bytes of 32 different rows at a time, took as long as the main loop (2,048 x 24,576 x
+// 4,096: 90 us with it, 64 without any stores).  16-byte piece c of row r lies at r * 128 + ((c ^ (r % 8)) * 16), off the banks of
+// its neighbours both ways.
 template <int EPI>
-__device__ __forceinline__ void f4_store_row(const uint32_t (&v)[32], const F4Args& p, int row, int col) {
+__device__ __forceinline__ void f4_store_rows(const uint32_t (&v0)[32], const uint32_t (&v1)[32], unsigned char* stage, const F4Args& p,
+                                              int row0, int col, int lane) {
   using OutT = typename std::conditional<EPI == 0, __nv_bfloat16, float>::type;
-  OutT* dst = (OutT*)p.out + (size_t)row * p.ldc + col;
-  if (col + 32 <= p.N && ((uintptr_t)dst & 15) == 0) {
+  constexpr int PER = 16 / sizeof(OutT);  // values of a piece
 #pragma unroll
-    for (int j = 0; j < 32 * (int)sizeof(OutT) / 16; ++j) {
-      if (EPI == 0)
-        reinterpret_cast<uint4*>(dst)[j] = make_uint4(pack2(v[8 * j], v[8 * j + 1]), pack2(v[8 * j + 2], v[8 * j + 3]),
-                                                      pack2(v[8 * j + 4], v[8 * j + 5]), pack2(v[8 * j + 6], v[8 * j + 7]));
-      else
-        reinterpret_cast<uint4*>(dst)[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  for (int c = 0; c < 8; ++c) {
+    uint4 x;
+    if (EPI == 0) {
+      const uint32_t(&v)[32] = c < 4 ? v0 : v1;
+      const int i = 8 * (c % 4);
+      x = make_uint4(pack2(v[i], v[i + 1]), pack2(v[i + 2], v[i + 3]), pack2(v[i + 4], v[i + 5]), pack2(v[i + 6], v[i + 7]));
+    } else {
+      x = make_uint4(v0[4 * c], v0[4 * c + 1], v0[4 * c + 2], v0[4 * c + 3]);
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (col + j < p.N) dst[j] = from_float<OutT>(__uint_as_float(v[j]));
+    *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = x;
   }
+  __syncwarp();
+  const int c = lane & 7, at = col + c * PER;
+  OutT* dst = (OutT*)p.out + (size_t)(row0 + (lane >> 3)) * p.ldc + at;
+  const bool whole = at + PER <= p.N && (((uintptr_t)p.out | (size_t)p.ldc * sizeof(OutT)) & 15) == 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i, dst += 4 * p.ldc) {
+    const int r = 4 * i + (lane >> 3);
+    const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
+    if (row0 + r < p.T) {
+      if (whole) {
+        *reinterpret_cast<uint4*>(dst) = x;
+      } else {
+        const OutT* e = reinterpret_cast<const OutT*>(&x);
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (at + j < p.N) dst[j] = e[j];
+      }
+    }
+  }
+  __syncwarp();
 }
-// 128 columns, gate and up in blocks of eight: two blocks of 32 results, their codes and two scales.
-__device__ __forceinline__ void f4_gated_row(const uint32_t (&v)[4][32], const F4Args& p, int row, int col) {
-  const int inner = p.N / 2, blocks = (inner + FP4_BLOCK - 1) / FP4_BLOCK, out_across = fp4_tiles(inner);
-  uint8_t* word = p.out_scales + fp4_scale_word(row, col / 256, out_across);
+// 64 columns, gate and up in blocks of eight: a block of 32 results, their codes and scale.
+__device__ __forceinline__ void f4_gated_block(const uint32_t (&v0)[32], const uint32_t (&v1)[32], const F4Args& p, int row, int col) {
+  const int inner = p.N / 2, blocks = (inner + FP4_BLOCK - 1) / FP4_BLOCK, out_across = fp4_tiles(inner), j = col / 64;
+  float gate[32], up[32], a[32];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int j = col / 64 + h;
-    float gate[32], up[32], a[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const int c = i / 8 * 16 + i % 8;
-      gate[i] = __uint_as_float(v[2 * h + c / 32][c % 32]);
-      up[i] = __uint_as_float(v[2 * h + (c + 8) / 32][(c + 8) % 32]);
-    }
-    f4_gate<32>(gate, up, p.act, a);
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      if (j * 32 + i >= inner) a[i] = 0.f;
-      top = max(top, __float_as_uint(a[i]) & 0x7fffffffu);
-    }
-    const uint32_t byte = fp4_scale_byte(top);
-    const float inv = fp4_inverse_scale(byte);
-    uint32_t w[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float s8[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s8[i] = a[8 * q + i] * inv;
-      w[q] = byte == 255u ? 0u : fp4_pack8(s8);
-    }
-    if (j < blocks) *reinterpret_cast<uint4*>(p.out_codes + (size_t)row * fp4_pitch(inner) + j * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-    word[j % 4] = (uint8_t)byte;  // beyond the last block: zero
-    if (col + 128 >= p.N && j % 4 < 2) word[j % 4 + 2] = 0;  // and so up to the end of the tile of scales
+  for (int i = 0; i < 32; ++i) {
+    const int c = i / 8 * 16 + i % 8;
+    gate[i] = __uint_as_float(c < 32 ? v0[c % 32] : v1[c % 32]);
+    up[i] = __uint_as_float(c < 32 ? v0[(c + 8) % 32] : v1[(c + 8) % 32]);
   }
+  f4_gate<32>(gate, up, p.act, a);
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    if (j * 32 + i >= inner) a[i] = 0.f;
+    top = max(top, __float_as_uint(a[i]) & 0x7fffffffu);
+  }
+  const uint32_t byte = fp4_scale_byte(top);
+  const float inv = fp4_inverse_scale(byte);
+  uint32_t w[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float s8[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s8[i] = a[8 * q + i] * inv;
+    w[q] = byte == 255u ? 0u : fp4_pack8(s8);
+  }
+  *reinterpret_cast<uint4*>(p.out_codes + (size_t)row * fp4_pitch(inner) + j * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+  uint8_t* word = p.out_scales + fp4_scale_word(row, j / 4, out_across);
+  word[j % 4] = (uint8_t)byte;
+  if (j + 1 == blocks)  // and the scales behind the last block, up to the end of their tile, are zero
+    for (int i = j % 4 + 1; i < 4; ++i) word[i] = 0;
 }
 
 // ---------------------------------------------------------------- a few tokens: small tiles, k shared out
@@ -220,14 +239,14 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   if (!aligned && threadIdx.x == 0) atomicOr(status, Q3_STATUS_TIMEOUT);
 
   auto scale_bytes = [&](int it) { return (uint32_t)min(2, across - 2 * (k0 + it)) * FP4_TILE_BYTES; };  // the last stage may have one tile
+  auto w_scales_at = [&](int it, int j) { return p.w_scales + ((size_t)(w_tile + j) * across + 2 * (k0 + it)) * FP4_TILE_BYTES; };
   auto load_w = [&](int it, int s) {
     unsigned char* b = smem_raw + (size_t)s * stage_bytes + shape.a_bytes();
     unsigned char* sb = b + shape.b_bytes() + 2 * FP4_TILE_BYTES;
     const uint32_t sf = scale_bytes(it);
     mbar_expect_tx(&full[s], shape.a_bytes() + shape.b_bytes() + (1 + w_here) * sf);
     tma_load_2d(b, &map_w, &full[s], (k0 + it) * 64, n0);
-    for (int j = 0; j < w_here; ++j)
-      f4_bulk_load(sb + j * 2 * FP4_TILE_BYTES, p.w_scales + ((size_t)(w_tile + j) * across + 2 * (k0 + it)) * FP4_TILE_BYTES, sf, &full[s]);
+    for (int j = 0; j < w_here; ++j) f4_bulk_load(sb + j * 2 * FP4_TILE_BYTES, w_scales_at(it, j), sf, &full[s]);
   };
   auto load_x = [&](int it, int s) {
     unsigned char* a = smem_raw + (size_t)s * stage_bytes;
@@ -236,10 +255,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     if (it != tc_drop_copy)  // tests of the give-up path only (see tc_common.cuh)
       tma_load_2d(a, &map_x, &full[s], (k0 + it) * 64, m0);
   };
-  int ahead = 0;  // thread 0: how many of its first stages are under way before the roles begin
   if (threadIdx.x == 0) {
-    tma_prefetch_map(&map_x);
-    tma_prefetch_map(&map_w);
     abort_flag = 0;
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
@@ -248,32 +264,25 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     mbar_init(acc_full, 1);
     mbar_init(sums_full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (early && aligned)  // the launch before this one did not write w: its part of the ring's first round goes out now
-      for (; ahead < min(stages, k_count); ++ahead) load_w(ahead, ahead);
     // the rows that this block finishes, from every block of the cluster
     if (split > 1) mbar_expect_tx(sums_full, (uint32_t)(split * (((rows_here - rank + split - 1) * shape.split_inverse) >> 16) * bn * 4));
   }
-  __syncwarp();
-  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for before anything is sent
-  pdl_wait();  // x comes from the kernel before this one
-  pdl_launch_dependents();
-  if (threadIdx.x == 0)
-    for (int it = 0; it < ahead; ++it) load_x(it, it);
-  // Tensor memory is taken only after the wait: a block that holds some while it waits for the kernel before it could keep
-  // that kernel's own blocks from ever getting theirs.
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(tmem_holder)), "r"(F4_FEW_COLS)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  tcgen05_fence_before();
   __syncthreads();
-  tcgen05_fence_after();
-  const uint32_t tmem = *tmem_holder;
+  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for before anything is sent
 
   if (warp == 0) {
+    // Where the launch before this one did not write w, its part of the ring's first round goes out ahead of the wait.
+    const int ahead = early ? min(stages, k_count) : 0;
+    if (aligned && elect_one()) {
+      tma_prefetch_map(&map_x);
+      for (int it = 0; it < ahead; ++it) load_w(it, it);
+    }
+    __syncwarp();
+    pdl_wait();  // x comes from the kernel before this one
     if (aligned) {
-      ahead = __shfl_sync(0xffffffffu, ahead, 0);
+      if (elect_one())
+        for (int it = 0; it < ahead; ++it) load_x(it, it);
+      __syncwarp();
       int it = ahead, s = ahead == stages ? 0 : ahead;
       for (uint32_t parity = 1; it < k_count; ++it) {
         if (it >= stages && !warp_wait(&empty[s], parity ^ 1, &abort_flag)) {
@@ -297,6 +306,14 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       __syncwarp();
     }
   } else if (warp == 1) {
+    pdl_wait();
+    pdl_launch_dependents();
+    // Tensor memory is taken only after the wait: a block that holds some while it waits for the kernel before it could keep
+    // that kernel's own blocks from ever getting theirs.
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(tmem_holder)), "r"(F4_FEW_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    const uint32_t tmem = *(volatile uint32_t*)tmem_holder;
     if (aligned) {
       bool ok = true;
       const uint32_t low = f4_idesc(bn, 0), high = f4_idesc(bn, 2);
@@ -338,6 +355,8 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       }
       __syncwarp();
     }
+  } else {
+    pdl_wait();
   }
   // Every thread gets here, whatever was given up, so the cluster's barrier needs no bound.
   if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -352,7 +371,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       __syncwarp();
     } else if (quarter * 32 < rows_here) {
       tcgen05_fence_after();
-      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
+      const uint32_t acc = *(volatile uint32_t*)tmem_holder + ((uint32_t)(quarter * 32) << 16);
       const int slot = (row * shape.split_inverse) >> 16, owner = row - slot * split;  // row / split, row % split
       const uint32_t to = split > 1 ? cluster_addr(s_addr(received + (rank * shape.slots + slot) * bn), owner) : 0;
       const uint32_t bar = split > 1 ? cluster_addr(s_addr(sums_full), owner) : 0;
@@ -382,6 +401,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   tcgen05_fence_before();
   __syncthreads();
   if (warp == 1) {
+    const uint32_t tmem = *(volatile uint32_t*)tmem_holder;
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(F4_FEW_COLS) : "memory");
   }
@@ -462,21 +482,25 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   }
 }
 
-// ---------------------------------------------------------------- many tokens: 256 x 256 tiles by pairs of CTAs
-// The CTA of rank r holds rows 128 r .. of the x tile and of the w tile, rows 128 r .. of the accumulator, its own rows' scales
-// and all of the w tile's scales; the roles are those of gemm_tc_pair_kernel (gemm_tc.cu).  An accumulator of 256 columns and
-// 24 columns of scales leave no room for a second accumulator, so the epilogue's warps take their 128 columns of a row into
-// registers at once and hand the accumulator back before they work on them.
+// ---------------------------------------------------------------- many tokens: 256 x 192 or 256 x 256 tiles by pairs of CTAs
+// The CTA of rank r holds rows 128 r .. of the x tile and half of the w tile's rows, rows 128 r .. of the accumulator, its own rows'
+// scales and all of the w tile's scales; the roles are those of gemm_tc_pair_kernel (gemm_tc.cu).  Tensor memory has room for two
+// accumulators of 192 columns beside the scales, and the epilogue of one tile runs under the main loop of the next; of 256
+// columns it has one, whose epilogue takes its columns into registers at once and hands it back, some 1,400 clocks in which the
+// tensor cores stand still.  The wider tile needs less operand traffic for its work and fits some sizes in fewer rounds.
+template <int BN, int EPI>
 struct F4Pair {
-  static constexpr int STAGES = 6;
-  static constexpr int A_BYTES = 128 * 128, B_BYTES = 128 * 128, SA_BYTES = 2 * FP4_TILE_BYTES, SB_BYTES = 4 * FP4_TILE_BYTES;
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;  // 35 KB
-  static constexpr size_t SMEM_BYTES = (size_t)STAGES * STAGE_BYTES + F4_BAR_BYTES;
-  static constexpr int EPI_WARPS = 8;
-  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr uint32_t COLS = 512;
-  static constexpr int GROUP = 8;  // tiles of x that are walked through for one tile of w before the next one
+  static constexpr int ACCS = BN == 192 ? 2 : 1;
+  static constexpr int STORE_BYTES = EPI == 2 ? 0 : 8 * 4096;  // where each of the epilogue's warps turns its rows around
+  static constexpr int STAGES = (BN == 192 ? 7 : 6) - (EPI == 2 ? 0 : 1);
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128, SA_BYTES = 2 * FP4_TILE_BYTES, SB_BYTES = 4 * FP4_TILE_BYTES;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;
+  static constexpr size_t SMEM_BYTES = (size_t)STAGES * STAGE_BYTES + STORE_BYTES + F4_BAR_BYTES;
+  static constexpr uint32_t SCALE_COL = ACCS * BN, COLS = 512;
 };
+constexpr int F4_PAIR_EPI_WARPS = 8;
+constexpr int F4_PAIR_THREADS = 64 + 32 * F4_PAIR_EPI_WARPS;
+constexpr int F4_PAIR_GROUP = 8;  // tiles of x that are walked through for one tile of w before the next one
 
 __device__ __forceinline__ void f4_mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t acc) {
   asm volatile(
@@ -493,31 +517,31 @@ __device__ __forceinline__ void f4_copy_scales_pair(uint32_t tmem, uint64_t desc
 
 // Tile number `i` of a walk over m_tiles x n_tiles in which GROUP tiles of x stay in the second-level cache.
 __device__ __forceinline__ void f4_tile(int i, int m_tiles, int n_tiles, int* m, int* n) {
-  const int per = F4Pair::GROUP * n_tiles, g = i / per, first = g * F4Pair::GROUP;
-  const int high = min(F4Pair::GROUP, m_tiles - first), j = i - g * per;
+  const int per = F4_PAIR_GROUP * n_tiles, g = i / per, first = g * F4_PAIR_GROUP;
+  const int high = min(F4_PAIR_GROUP, m_tiles - first), j = i - g * per;
   *m = first + j % high;
   *n = j / high;
 }
 
-template <int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F4Pair::THREADS)
+template <int EPI, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F4_PAIR_THREADS)
 gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_ws,
                      const __grid_constant__ F4Args p, int* status) {
-  using S = F4Pair;
+  using S = F4Pair<BN, EPI>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw + (size_t)S::STAGES * S::STAGE_BYTES);  // used in rank 0
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw + (size_t)S::STAGES * S::STAGE_BYTES + S::STORE_BYTES);  // used in rank 0
   uint64_t* empty = full + S::STAGES;
   uint64_t* acc_full = empty + S::STAGES;
-  uint64_t* acc_empty = acc_full + 1;  // used in rank 0
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 1);
+  uint64_t* acc_empty = acc_full + S::ACCS;  // used in rank 0
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + S::ACCS);
   __shared__ int abort_flag;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int across = fp4_tiles(p.K), k_stages = (across + 1) / 2;
-  const int m_tiles = (p.T + 255) / 256, n_tiles = (p.N + 255) / 256;
+  const int m_tiles = (p.T + 255) / 256, n_tiles = (p.N + BN - 1) / BN;
   const bool aligned = (s_addr(smem_raw) & 1023u) == 0;  // the same in both CTAs
   const int num_tiles = aligned ? m_tiles * n_tiles : 0;
   if (!aligned && threadIdx.x == 0) atomicOr(status, Q3_STATUS_TIMEOUT);
@@ -538,8 +562,10 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 2 * S::EPI_WARPS);  // the epilogue warps of both CTAs
+    for (int b = 0; b < S::ACCS; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * F4_PAIR_EPI_WARPS);  // the epilogue warps of both CTAs
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
@@ -575,8 +601,8 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         const uint32_t bar = cluster_addr(s_addr(&full[s]), 0);
         if (elect_one()) {
           if (rank == 0) mbar_expect_tx(&full[s], 2 * S::STAGE_BYTES);
-          tma_load_2d_pair(b, &map_w, bar, kt * 64, n * 256 + (int)rank * 128);
-          tma_load_2d_pair(sb, &map_ws, bar, kt * 256, n * 2);
+          tma_load_2d_pair(b, &map_w, bar, kt * 64, n * BN + (int)rank * (BN / 2));
+          tma_load_2d_pair(sb, &map_ws, bar, kt * 256, n * BN / FP4_TILE);
           tma_load_2d_pair(sa, &map_xs, bar, kt * 256, m * 2 + (int)rank);
           if ((int)it != tc_drop_copy || rank != 0)  // tests of the give-up path only (see tc_common.cuh)
             tma_load_2d_pair(a, &map_x, bar, kt * 64, m * 256 + (int)rank * 128);
@@ -590,7 +616,10 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
       uint32_t it = 0, t = 0;
       bool ok = true;
       for (int tile = pair; tile < num_tiles && ok; tile += pairs, ++t) {
-        if (t > 0 && !warp_wait_cluster(acc_empty, (t & 1) ^ 1, &abort_flag)) {
+        int m, n;
+        f4_tile(tile, m_tiles, n_tiles, &m, &n);
+        const uint32_t buf = t % S::ACCS, acc = tmem + buf * BN, shift = n * BN % FP4_TILE / 32;  // of its scales: a column per 32 rows
+        if (t >= S::ACCS && !warp_wait_cluster(&acc_empty[buf], ((t / S::ACCS) & 1) ^ 1, &abort_flag)) {
           ok = false;
           break;
         }
@@ -606,7 +635,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
           const unsigned char *b = a + S::A_BYTES, *sa = b + S::B_BYTES, *sb = sa + S::SA_BYTES;
           const uint64_t a_desc = umma_desc_sw128(a), b_desc = umma_desc_sw128(b), sa_desc = f4_scale_desc(sa), sb_desc = f4_scale_desc(sb);
           // the scales of this stage beside those of the last one, which its instructions may still read
-          const uint32_t ta = tmem + 256 + (it & 1) * 24, tb = ta + 8;
+          const uint32_t ta = tmem + S::SCALE_COL + (it & 1) * 24, tb = ta + 8;
           const bool both = across - 2 * kt > 1;
           if (elect_one()) {
 #pragma unroll
@@ -615,11 +644,11 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                 f4_copy_scales_pair(ta + 4 * h, sa_desc + h * (FP4_TILE_BYTES >> 4));
                 f4_copy_scales_pair(tb + 8 * h, sb_desc + h * (FP4_TILE_BYTES >> 4));
                 f4_copy_scales_pair(tb + 8 * h + 4, sb_desc + (S::SA_BYTES >> 4) + h * (FP4_TILE_BYTES >> 4));
-                f4_mma_pair(tmem, a_desc + 4 * h, b_desc + 4 * h, f4_idesc(256, 0, 256), ta + 4 * h, tb + 8 * h, (kt | h) != 0);
-                f4_mma_pair(tmem, a_desc + 4 * h + 2, b_desc + 4 * h + 2, f4_idesc(256, 2, 256), ta + 4 * h, tb + 8 * h, 1);
+                f4_mma_pair(acc, a_desc + 4 * h, b_desc + 4 * h, f4_idesc(BN, 0, 256), ta + 4 * h, tb + shift + 8 * h, (kt | h) != 0);
+                f4_mma_pair(acc, a_desc + 4 * h + 2, b_desc + 4 * h + 2, f4_idesc(BN, 2, 256), ta + 4 * h, tb + shift + 8 * h, 1);
               }
             umma_commit_pair(&empty[s]);
-            if (kt + 1 == k_stages) umma_commit_pair(acc_full);
+            if (kt + 1 == k_stages) umma_commit_pair(&acc_full[buf]);
           }
           __syncwarp();
         }
@@ -627,35 +656,43 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
       if (!ok && lane == 0) give_up();
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    const uint32_t release = cluster_addr(s_addr(acc_empty), 0);
+    // two warps for each quarter of the rows: the first 128 columns and the others
+    const int quarter = warp & 3, half = (warp - 2) >> 2, chunks = half ? (BN - 128) / 32 : 4;
+    unsigned char* const store = smem_raw + (size_t)S::STAGES * S::STAGE_BYTES + (warp - 2) * 4096;  // EPI 0, 1
     uint32_t t = 0;
     for (int tile = pair; tile < num_tiles; tile += pairs, ++t) {
       int m, n;
       f4_tile(tile, m_tiles, n_tiles, &m, &n);
-      const bool ready = mbar_wait(acc_full, t & 1, &abort_flag);
-      if (!__all_sync(0xffffffffu, ready)) {
+      const uint32_t buf = t % S::ACCS;
+      if (!warp_wait(&acc_full[buf], (t / S::ACCS) & 1, &abort_flag)) {
         if (lane == 0) give_up();
+        __syncwarp();
         break;
       }
       tcgen05_fence_after();
-      const int row = m * 256 + (int)rank * 128 + quarter * 32 + lane, n0 = n * 256 + half * 128;
-      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)half * 128;
+      const int row0 = m * 256 + (int)rank * 128 + quarter * 32, n0 = n * BN + half * 128;
+      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN + (uint32_t)half * 128;
       uint32_t v[4][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32(acc + 32 * c, v[c]);
+      for (int c = 0; c < 4; ++c)
+        if (c < chunks) tmem_ld_32(acc + 32 * c, v[c]);
       tmem_wait_ld();
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(release);
-      if (row >= p.T || n0 >= p.N) continue;
-      if (EPI == 2) {
-        f4_gated_row(v, p, row, n0);
-      } else {
+      if (lane == 0) mbar_arrive_cluster(cluster_addr(s_addr(&acc_empty[buf]), 0));
+      __syncwarp();
+      if (row0 >= p.T) continue;  // uniform over the warp
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (n0 + 32 * c < p.N) f4_store_row<EPI>(v[c], p, row, n0 + 32 * c);
+      for (int c = 0; c < 4; c += 2) {
+        if (c >= chunks || n0 + 32 * c >= p.N) break;
+        if (EPI == 2) {
+          if (row0 + lane < p.T) f4_gated_block(v[c], v[c + 1], p, row0 + lane, n0 + 32 * c);
+        } else {
+          f4_store_rows<EPI>(v[c], v[c + 1], store, p, row0, n0 + 32 * c, lane);
+          if (EPI == 1 && n0 + 32 * c + 32 < p.N) f4_store_rows<EPI>(v[c + 1], v[c + 1], store, p, row0, n0 + 32 * c + 32, lane);
+        }
       }
+      __syncwarp();
     }
   }
   tcgen05_fence_before();
@@ -748,39 +785,74 @@ static F4FewShape f4_few_shape(int T, int N, int K) {
   best.split_inverse = (65536 + best.split - 1) / best.split;
   const int need = best.depth;
   const int alone = best.split > 1 ? 0 : rows * (best.bn + 4) * 4;  // the sums' place over the ring
-  // half of an SM's shared memory, so that a block of the next kernel fits beside; all of it where that leaves under three stages
-  for (int room = 112 * 1024;; room = 224 * 1024) {
+  // Up to eight stages a block keeps to half of an SM's shared memory, so that a block of the next kernel fits beside it and has its
+  // first stages on their way while this one ends (1 x 4,096 x 12,288, eight stages: 6.2 us in 112 KB, 7.2 in 224); where it works
+  // through more, a deeper ring does more for it (8 x 24,576 x 4,096, sixteen stages: 14.1 us in 112 KB, 12.2 in 160).  All of it
+  // where that leaves under three stages, or no place for the sums.
+  for (int room = need > 8 ? 160 * 1024 : 112 * 1024;; room = 224 * 1024) {
     best.stages = (room - best.received_bytes() - F4_BAR_BYTES) / best.stage_bytes();
     if (best.stages > need) best.stages = need;
     if (best.stages > F4_FEW_MAX_STAGES) best.stages = F4_FEW_MAX_STAGES;
     if (best.stages < 1) best.stages = 1;
-    if (room > 112 * 1024 || ((best.stages >= 3 || best.stages == need) && best.ring_bytes() >= alone)) break;
+    if (room > 160 * 1024 || ((best.stages >= 3 || best.stages == need) && best.ring_bytes() >= alone)) break;
   }
   while (best.ring_bytes() < alone) ++best.stages;
   return best;
 }
 
-template <int EPI>
-static int gemm_fp4_pair_launch(const CUtensorMap& map_x, const CUtensorMap& map_w, const F4Args& p, int* status, cudaStream_t stream) {
+// How many pairs of CTAs the device runs at a time (a cluster's two CTAs need SMs of one group).
+static int f4_pair_slots() {
+  static int slots[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+  if (slots[dev] == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * sm_count());
+    cfg.blockDim = dim3(F4_PAIR_THREADS);
+    cfg.dynamicSmemBytes = F4Pair<256, 0>::SMEM_BYTES;
+    int n = 0;
+    if (cudaFuncSetAttribute(gemm_fp4_pair_kernel<0, 256>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F4Pair<256, 0>::SMEM_BYTES) !=
+            cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, gemm_fp4_pair_kernel<0, 256>, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = sm_count() / 2;
+    }
+    slots[dev] = n < sm_count() / 2 ? n : sm_count() / 2;
+  }
+  return slots[dev];
+}
+
+// Clocks of the pair kernel's rounds, from measured times: a stage of 192 or 256 columns takes 410 or 522, a tile of 256 a further
+// 1,400.  (192 and 256 columns: 78 and 81 us at 2,048 x 24,576 x 4,096, 44 and 41 at 2,048 x 4,096 x 12,288, 359 and 352 at 8,192 x
+// 5,120 x 25,600.)
+static double f4_pair_cost(int T, int N, int K, int bn) {
+  const long long tiles = (long long)((N + bn - 1) / bn) * ((T + 255) / 256), slots = f4_pair_slots();
+  const int k_stages = (fp4_tiles(K) + 1) / 2;
+  return (double)((tiles + slots - 1) / slots) * (bn == 192 ? k_stages * 410.0 : k_stages * 522.0 + 1400.0);
+}
+
+template <int EPI, int BN>
+static int gemm_fp4_pair_launch(const void* x_codes, const void* w_codes, const F4Args& p, int* status, cudaStream_t stream) {
+  using S = F4Pair<BN, EPI>;
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(gemm_fp4_pair_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F4Pair::SMEM_BYTES);
-    if (e == cudaSuccess)  // a kernel that asks for less keeps its SM from taking a block of one that asks for more beside its own
-      e = cudaFuncSetAttribute(gemm_fp4_pair_kernel<EPI>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    cudaError_t e = cudaFuncSetAttribute(gemm_fp4_pair_kernel<EPI, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM_BYTES);
     if (e != cudaSuccess) return (int)e;
     configured = true;
   }
-  CUtensorMap map_xs, map_ws;
-  const uint64_t across = fp4_tiles(p.K);
-  int code = f4_scale_map(&map_xs, p.x_scales, fp4_tiles(p.T), across, 1);
+  // the maps of codes take two bytes as one bfloat16: only bytes move
+  CUtensorMap map_x, map_w, map_xs, map_ws;
+  const uint64_t cols = fp4_pitch(p.K) / 2, across = fp4_tiles(p.K);
+  int code = cached_map(&map_x, x_codes, (uint64_t)p.T, cols, 128);
+  if (!code) code = cached_map(&map_w, w_codes, (uint64_t)p.N, cols, BN / 2);
+  if (!code) code = f4_scale_map(&map_xs, p.x_scales, fp4_tiles(p.T), across, 1);
+  if (!code) code = f4_scale_map(&map_ws, p.w_scales, fp4_tiles(p.N), across, 2);
   if (code) return code;
-  code = f4_scale_map(&map_ws, p.w_scales, fp4_tiles(p.N), across, 2);
-  if (code) return code;
-  const long long tiles = (long long)((p.N + 255) / 256) * ((p.T + 255) / 256);
+  const long long tiles = (long long)((p.N + BN - 1) / BN) * ((p.T + 255) / 256);
   if (tiles > 0x3fffffffLL) return Q3_ERR_SIZE;
-  const long long slots = sm_count() / 2;
-  code = f4_launch(gemm_fp4_pair_kernel<EPI>, dim3((unsigned)(2 * (tiles < slots ? tiles : slots))), F4Pair::THREADS,
-                   F4Pair::SMEM_BYTES, 1, stream, map_x, map_w, map_xs, map_ws, p, status);
+  const long long slots = f4_pair_slots();
+  code = f4_launch(gemm_fp4_pair_kernel<EPI, BN>, dim3((unsigned)(2 * (tiles < slots ? tiles : slots))), F4_PAIR_THREADS, S::SMEM_BYTES,
+                   1, stream, map_x, map_w, map_xs, map_ws, p, status);
   const int last = launch_status();
   return code ? code : last;
 }
@@ -788,18 +860,19 @@ static int gemm_fp4_pair_launch(const CUtensorMap& map_x, const CUtensorMap& map
 // early: w was not written by the launch before this one.
 template <int EPI>
 static int gemm_fp4(const void* x_codes, const void* w_codes, const F4Args& p, int early, int* status, cudaStream_t stream) {
-  const int sms = sm_count();
-  const bool pair = p.T > 256 && (long long)((p.T + 255) / 256) * ((p.N + 255) / 256) >= sms / 4;
-  F4FewShape shape{};
-  if (!pair) shape = f4_few_shape(p.T, p.N, p.K);
+  if (p.T > 256 && (long long)((p.T + 255) / 256) * ((p.N + 255) / 256) >= sm_count() / 4) {
+    if (f4_pair_cost(p.T, p.N, p.K, 192) <= f4_pair_cost(p.T, p.N, p.K, 256))
+      return gemm_fp4_pair_launch<EPI, 192>(x_codes, w_codes, p, status, stream);
+    return gemm_fp4_pair_launch<EPI, 256>(x_codes, w_codes, p, status, stream);
+  }
+  const F4FewShape shape = f4_few_shape(p.T, p.N, p.K);
   // the maps take two bytes of codes as one bfloat16: only bytes move
   CUtensorMap map_x, map_w;
   const uint64_t cols = fp4_pitch(p.K) / 2;
-  int code = cached_map(&map_x, x_codes, (uint64_t)p.T, cols, pair ? 128 : shape.a_rows);
+  int code = cached_map(&map_x, x_codes, (uint64_t)p.T, cols, shape.a_rows);
   if (code) return code;
-  code = cached_map(&map_w, w_codes, (uint64_t)p.N, cols, pair ? 128 : shape.bn);
+  code = cached_map(&map_w, w_codes, (uint64_t)p.N, cols, shape.bn);
   if (code) return code;
-  if (pair) return gemm_fp4_pair_launch<EPI>(map_x, map_w, p, status, stream);
   return gemm_fp4_few_launch<EPI>(map_x, map_w, p, shape, early, status, stream);
 }
 
