@@ -37,9 +37,6 @@ __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t top) {
 }
 // 1 / X.  b is at most 253, so this is a normal number; 255 gives 0, which leaves zeros (and NaN) for the codes.
 __device__ __forceinline__ float fp4_inverse_scale(uint32_t b) { return b == 255u ? 0.f : __uint_as_float((254u - b) << 23); }
-__device__ __forceinline__ float fp4_scale(uint32_t b) {
-  return __uint_as_float(b == 0u ? 0x00400000u : (b == 255u ? 0x7fc00000u : b << 23));
-}
 
 // Eight values, already divided by their scale, as codes: value i in bits 4 i .. 4 i + 3.
 __device__ __forceinline__ uint32_t fp4_pack8(const float (&v)[8]) {
@@ -59,17 +56,6 @@ __device__ __forceinline__ uint32_t fp4_pack2(float lo, float hi) {
   asm("{\n\t.reg .b8 a;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tmov.b32 %0, {a, a, a, a};\n\t}" : "=r"(r) : "f"(lo), "f"(hi));
   return r & 255u;
 }
-// What two codes (the low eight bits) stand for, before their scale.
-__device__ __forceinline__ float2 fp4_pair(uint32_t two) {
-  uint32_t h;
-  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(h) : "r"(two));
-  float2 f;
-  asm("{\n\t.reg .f16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}"
-      : "=f"(f.x), "=f"(f.y)
-      : "r"(h));
-  return f;
-}
-
 // Eight values of a row in each of four neighbouring lanes, a block between them: their codes, and the block's scale.  Every
 // lane of the warp takes part.
 __device__ __forceinline__ uint32_t fp4_round8(const float (&v)[8], uint32_t* scale_byte) {
