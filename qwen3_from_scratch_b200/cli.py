@@ -43,6 +43,8 @@ def _add_engine_options(p: argparse.ArgumentParser) -> None:
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--random-weights", action="store_true",
                    help="--model needs only config.json: weights are drawn on the device from --seed")
+    p.add_argument("--feed-forward-weights", choices=["fp4"], default=None,
+                   help="hold gated feed-forwards in microscaled 4-bit floating point (not with --config-path)")
     p.add_argument("--ignore-eos", action="store_true")
     p.add_argument("--eos-token-id", type=int, default=None)
     p.add_argument("--log-interval", type=int, default=0)
@@ -62,7 +64,8 @@ def _engine(args):
                       chunked_prefill_size=args.chunked_prefill_size, temperature=args.temperature,
                       top_k=args.top_k, max_new_tokens=args.max_new_tokens, seed=args.seed,
                       eos_token_id=args.eos_token_id, log_interval=args.log_interval,
-                      random_weights=args.seed if args.random_weights else None)
+                      random_weights=args.seed if args.random_weights else None,
+                      feed_forward_weights=args.feed_forward_weights)
 
 
 def cmd_generate(args) -> int:

@@ -84,11 +84,12 @@ class SyncEngine:
                  chunked_prefill_size: int = 512, enable_prefix_cache: bool = False,
                  temperature: float = 0.0, top_k: int = 0, max_new_tokens: int = 100, seed: int = 0,
                  eos_token_id: Optional[int] = None, log_interval: int = 0, cuda_graphs: bool = True,
-                 lookahead: bool = True, random_weights: Optional[int] = None):
+                 lookahead: bool = True, random_weights: Optional[int] = None, feed_forward_weights: Optional[str] = None):
         """``random_weights``: a seed; ``model_path`` then needs only config.json and the weights are drawn on
         the device.  ``num_pages`` fixes the size of the cache pool; otherwise ``gpu_utilization`` of the
         memory that is free after the weights are loaded is given to it.  ``lookahead``: while a plain
-        decode step runs, the step after it is already put on the device (see ``step``)."""
+        decode step runs, the step after it is already put on the device (see ``step``).  ``feed_forward_weights``: see
+        ``Session``."""
         if enable_prefix_cache:
             # The reference's own configurations set this (its default is true: factory/batch_config.py:147).
             # Sharing pages between requests with a common prefix saves work and changes no output, so the
@@ -105,7 +106,8 @@ class SyncEngine:
                                                   max_num_seqs)
         self.session = Session(model_path, dtype=dtype, device=device, page_size=block_size,
                                num_pages=cache_pages, max_seqs=max_num_seqs, max_step_tokens=max_num_tokens,
-                               cuda_graphs=cuda_graphs, random_weights=random_weights)
+                               cuda_graphs=cuda_graphs, random_weights=random_weights,
+                               feed_forward_weights=feed_forward_weights)
         self.config = self.session.config
         spec = self.session.model.spec
         self.eos_token_id = eos_token_id if eos_token_id is not None else spec.eos_token_id

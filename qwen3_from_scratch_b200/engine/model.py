@@ -131,10 +131,11 @@ class Model:
         return self.head.forward(wanted)
 
 
-def load_model(folder: str, dtype, device, max_tokens: int, max_seqs: int, random_weights: Optional[int] = None):
+def load_model(folder: str, dtype, device, max_tokens: int, max_seqs: int, random_weights: Optional[int] = None,
+               feed_forward_weights: Optional[str] = None):
     """config.json -> configuration -> specification -> parts -> weights on the device.
     Returns (model, configuration, runtime).  ``random_weights``: a seed; the folder then needs only its
-    config.json and the weights are drawn on the device instead of read."""
+    config.json and the weights are drawn on the device instead of read.  ``feed_forward_weights``: see ``Runtime``."""
     if not torch.cuda.is_available():
         raise RuntimeError("this engine runs on a CUDA GPU (sm_100a); no GPU is visible")
     ops.library()  # build or load the kernels first: without them nothing below can run
@@ -142,7 +143,8 @@ def load_model(folder: str, dtype, device, max_tokens: int, max_seqs: int, rando
     model = Model(build_model_spec(config))
     compute = resolve_dtype(dtype)
     device = torch.device(device)
-    rt = Runtime(device=device, dtype=compute, max_tokens=int(max_tokens), max_seqs=int(max_seqs))
+    rt = Runtime(device=device, dtype=compute, max_tokens=int(max_tokens), max_seqs=int(max_seqs),
+                 feed_forward_weights=feed_forward_weights)
     if random_weights is not None:
         weights = random_weights_on_device(model.weight_specs(), int(random_weights), device, compute)
     else:

@@ -132,10 +132,14 @@ class Runtime:
     dtype: torch.dtype
     max_tokens: int
     max_seqs: int
+    #: how gated feed-forwards hold their weights: None (as the checkpoint has them) or "fp4" (rows of microscaled 4-bit values)
+    feed_forward_weights: Optional[str] = None
     status: torch.Tensor = None  # int32[1] on the device; kernels OR error bits into it
     mailbox: torch.Tensor = None  # int32[1 + max_seqs]: the status word, then a step's sampled tokens
 
     def __post_init__(self):
+        if self.feed_forward_weights not in (None, "fp4"):
+            raise ValueError(f"feed-forward weights are held as they are (None) or as 'fp4', not {self.feed_forward_weights!r}")
         if self.status is None:
             # the status word and the sampled tokens lie side by side, so that one read brings both
             self.mailbox = torch.zeros(1 + max(1, self.max_seqs), dtype=torch.int32, device=self.device)

@@ -24,6 +24,7 @@ from ..kernels import ops
 from .base import (EMBEDDING_OUTPUT, EMBEDDING_SIDE, LAYER_REPEAT, NEXT_NORM_WEIGHT, STREAM_SUMSQ, Block, PartSpec, PendingNormed,
                    PendingStreamWrite, PendingSum, PendingTerm, Runtime, StateSpec, StepContext, WeightSpec)
 from .linear import Linear
+from .norm import RMSNorm
 
 
 @register_part("block", "pre_norm")
@@ -157,6 +158,9 @@ class PreNormBlock(Block):
         a = self.mixer.forward(x, ctx, cache_id, write_cache)
         if self.feed_forward is None:
             return a
+        if (getattr(self.feed_forward, "reads_stream", False) and self.conv_taps is None and type(self.norm2) is RMSNorm
+                and (a is None or isinstance(a, torch.Tensor))):
+            return self.feed_forward.from_stream(stream, a, self.norm2.weight, self.norm2.eps)
         x = self._read(1, self.norm2, stream, a, ctx, cache_id)
         return self.feed_forward.forward(x)
 

@@ -5,6 +5,9 @@ as parameters.
 
 Reference: models/feedback.py:14-34.  The gate and up weights are merged into one [2I, H] weight at load, so
 one product feeds the gate kernel.
+
+Where the run asks for it (``Runtime.feed_forward_weights = "fp4"``) a gated feed-forward holds its weights in microscaled 4-bit
+floating point and rounds what its products read in the same way.
 """
 
 from __future__ import annotations
@@ -54,6 +57,9 @@ class GatedMLP(FeedForward):
 
     def setup(self, rt: Runtime, weights: Dict[str, torch.Tensor]) -> None:
         super().setup(rt, weights)
+        self.fp4 = rt.feed_forward_weights == "fp4"
+        if self.fp4:
+            return self._setup_fp4(rt, weights)
         gate = weights.pop(self.tensors["gate"])
         up = weights.pop(self.tensors["up"])
         dtype = torch.float32 if torch.float32 in (gate.dtype, up.dtype) else gate.dtype
@@ -81,13 +87,57 @@ class GatedMLP(FeedForward):
         # product that also applies a norm that was never computed is built for the SiLU gate
         self.fused_gate = self.blocks_of_eight
 
+    def _setup_fp4(self, rt: Runtime, weights: Dict[str, torch.Tensor]) -> None:
+        """Weights as ``ops.Fp4Rows``, gate and up rows alternating in blocks of eight, and room for the rounded activations."""
+        h, i = self.hidden_size, self.intermediate_size
+        if self.has_bias or self.activation not in ops.FP4_GATES or i % 8:
+            raise ValueError(f"feed-forward {self.name}: fp4 weights take no biases, one of {ops.FP4_GATES} as the gate and a width in "
+                             f"multiples of 8, not {self.activation}, {i}{' and biases' if self.has_bias else ''}")
+        gate, up = weights.pop(self.tensors["gate"]), weights.pop(self.tensors["up"])
+        merged = torch.cat([gate.view(i // 8, 8, h), up.view(i // 8, 8, h)], dim=1).reshape(2 * i, h)
+        del gate, up
+        self.gate_up4, self.down4 = ops.fp4_rows(2 * i, h, rt.device), ops.fp4_rows(h, i, rt.device)
+        ops.fp4_quantise(merged, self.gate_up4)
+        ops.fp4_quantise(weights.pop(self.tensors["down"]), self.down4)
+
+        def held(role: str, width: int) -> ops.Fp4Rows:
+            u8 = {"dtype": torch.uint8}
+            return ops.Fp4Rows(rt.shared(f"ffn.fp4.{role}.codes", rt.max_tokens, -(-width // 32) * 16, **u8),
+                               rt.shared(f"ffn.fp4.{role}.scales", -(-rt.max_tokens // 128), -(-width // 128), 512, **u8), width)
+
+        self._normed4, self._gated4 = held("normed", h), held("gated", i)
+        self._y = rt.shared("ffn.fp4.out", rt.max_tokens, h)
+
+    @property
+    def reads_stream(self) -> bool:
+        """Whether ``from_stream`` takes the place of the norm in front and ``forward``."""
+        return self.fp4
+
+    def from_stream(self, stream: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, eps: float) -> torch.Tensor:
+        """stream += delta; the feed-forward of rmsnorm(stream) * weight, whose rows are rounded as they leave the norm."""
+        rows = stream.shape[0]
+        y = self._y[:rows]
+        ops.fp4_feed_forward(stream, delta, weight, eps, self.gate_up4, self.down4, self._normed4.first(rows),
+                             self._gated4.first(rows), y, self.rt.status, activation=self.activation)
+        return y
+
+    def _forward_fp4(self, x: torch.Tensor) -> torch.Tensor:
+        rows = x.shape[0]
+        h, a, y = self._normed4.first(rows), self._gated4.first(rows), self._y[:rows]
+        ops.fp4_quantise(x, h)
+        ops.fp4_gated_product(h, self.gate_up4, a, self.rt.status, activation=self.activation)
+        ops.fp4_product(a, self.down4, y, self.rt.status)
+        return y
+
     fuses_stream = True
 
     def can_fuse_stream(self, rows: int) -> bool:
-        return (self.fused_gate and not self.has_bias and self.activation == "silu" and self.gate_up.takes_stream_norm(rows)
+        return not self.fp4 and (self.fused_gate and not self.has_bias and self.activation == "silu" and self.gate_up.takes_stream_norm(rows)
                 and self.down.can_add_into_stream(rows))
 
     def forward(self, x, into_stream=None, next_norm_weight=None):
+        if self.fp4:
+            return self._forward_fp4(x)
         act = self._act[: x.shape[0]]
         rows = x.shape[0]
         if isinstance(x, StreamNorm):
@@ -142,6 +192,8 @@ class DenseMLP(FeedForward):
 
     def setup(self, rt: Runtime, weights: Dict[str, torch.Tensor]) -> None:
         super().setup(rt, weights)
+        if rt.feed_forward_weights is not None:
+            raise ValueError(f"feed-forward {self.name}: {rt.feed_forward_weights} weights are built for gated feed-forwards only")
         self.up = Linear(weights.pop(self.tensors["up"]), rt, tag="ffn.up")
         self.down = Linear(weights.pop(self.tensors["down"]), rt, tag="ffn.down")
 
@@ -250,6 +302,8 @@ class RoutedExperts(FeedForward):
 
     def setup(self, rt: Runtime, weights: Dict[str, torch.Tensor]) -> None:
         super().setup(rt, weights)
+        if rt.feed_forward_weights is not None:
+            raise ValueError(f"feed-forward {self.name}: {rt.feed_forward_weights} weights are built for dense gated feed-forwards only")
         self.router = weights[f"{self.name}.{self.n['router']}"]
         self.correction = weights[f"{self.name}.{self.n['correction']}"] if self.has_correction else None
         self.router_bias = weights[f"{self.name}.{self.n['router_bias']}"] if self.has_router_bias else None

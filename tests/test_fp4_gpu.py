@@ -398,3 +398,50 @@ def test_a_wait_that_runs_out_is_given_up_cleanly(rows, features, width):
     o.fp4_product(x, w, y, st)
     assert int(st.item()) == 0
     assert bool(((y.cpu().double() - xv @ wv.t()).abs() <= product_tolerance(xv, wv)).all())
+
+
+# ---------------------------------------------------------------- a model whose feed-forwards are held so
+def plain_mlp(x, w, prefix):
+    """The feed-forward of the plain model with weights and activations rounded."""
+    h = plain.rounded(x.double())
+    gate = h @ plain.rounded(w[f"{prefix}.gate_proj.weight"].double()).t()
+    up = h @ plain.rounded(w[f"{prefix}.up_proj.weight"].double()).t()
+    a = plain.rounded(gate * torch.sigmoid(gate) * up)
+    return (a @ plain.rounded(w[f"{prefix}.down_proj.weight"].double()).t()).to(x.dtype)
+
+
+@pytest.mark.parametrize("key", ["a", "b", "d"])
+def test_model_with_fp4_feed_forwards(tiny_folders, monkeypatch, key):
+    """In float32, prompts whole and token by token.  The engine's float32 sums differ from the plain model's by about 1e-6, which
+    moves a value across a boundary between two codes once in some 10^5 of them (a test has 10^4) and nothing else by more than the
+    1e-5 of the float32 replays; a moved code would show as 1e-3 and more of the logits, so a tenth of that is the bound."""
+    import plain_qwen3
+    from conftest import TINY, random_tokens
+    from qwen3_from_scratch_b200.engine.batch import Entry
+    from qwen3_from_scratch_b200.engine.session import Session
+    folder = tiny_folders[key]
+    cfg, w = plain_qwen3.read_model_folder(folder)
+    ids = random_tokens(TINY[key][0]["vocab_size"], 20, 3)
+    without = plain_qwen3.forward_logits(cfg, w, ids)
+    monkeypatch.setattr(plain_qwen3, "swiglu_mlp", plain_mlp)
+    want = plain_qwen3.forward_logits(cfg, w, ids).double()
+    session = Session(folder, dtype="float32", page_size=8, num_pages=16, max_seqs=2, max_step_tokens=64, feed_forward_weights="fp4")
+    whole = session.step([Entry("r", ids, list(range(20)))]).cpu().double()
+    session.end("r")
+    rows = [session.step([Entry("s", [t], [0])]).cpu().double() for t in ids]
+    session.check_status()
+    scale = float(want.abs().max())
+    for got in (whole, torch.cat(rows)):
+        assert float((got - want).abs().max()) <= 1e-4 * scale
+    assert float((without.double() - want).abs().max()) > 1e-3 * scale  # the rounding is seen at all
+
+
+def test_engine_generates_with_fp4_feed_forwards(tiny_folders):
+    from qwen3_from_scratch_b200.engine.engine import SyncEngine
+    engine = SyncEngine(tiny_folders["d"], max_num_seqs=4, max_num_tokens=256, num_pages=64, max_new_tokens=12,
+                        feed_forward_weights="fp4")
+    first = [r.token_ids for r in engine.batch_generate([[1, 2, 3], list(range(5, 150))], ignore_eos=True)[0]]
+    again = [r.token_ids for r in engine.batch_generate([[1, 2, 3], list(range(5, 150))], ignore_eos=True)[0]]
+    assert first == again and [len(t) for t in first] == [12, 12]
+    with pytest.raises(ValueError, match="fp4"):
+        SyncEngine(tiny_folders["d"], num_pages=64, feed_forward_weights="int3")
