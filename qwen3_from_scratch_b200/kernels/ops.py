@@ -3217,20 +3217,20 @@ def fp4_quantise(x: torch.Tensor, out: Fp4Rows, values: Optional[torch.Tensor] =
 
 def _check_fp4_stream(name: str, stream: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor,
                       stream_out: Optional[torch.Tensor], dtype: torch.dtype) -> Tuple[int, int]:
+    size = stream.shape
     _check(f"{name}.stream", stream, torch.float32)
     _check(f"{name}.weight", weight, torch.float32)
-    T, H = stream.shape
+    if len(size) != 2 or weight.shape[-1] != size[1] or weight.numel() != size[1]:
+        raise KernelError(f"{name}: weight {tuple(weight.shape)}, stream {tuple(size)}")
     if delta is not None:
         _check(f"{name}.delta", delta, dtype)
-        if tuple(delta.shape) != (T, H):
-            raise KernelError(f"{name}: delta {tuple(delta.shape)} vs stream {(T, H)}")
+        if delta.shape != size:
+            raise KernelError(f"{name}: delta {tuple(delta.shape)} vs stream {tuple(size)}")
     if stream_out is not None:
         _check(f"{name}.stream_out", stream_out, torch.float32)
-        if tuple(stream_out.shape) != (T, H):
-            raise KernelError(f"{name}: stream_out {tuple(stream_out.shape)} vs stream {(T, H)}")
-    if weight.numel() != H:
-        raise KernelError(f"{name}: weight {tuple(weight.shape)}, stream {(T, H)}")
-    return T, H
+        if stream_out.shape != size:
+            raise KernelError(f"{name}: stream_out {tuple(stream_out.shape)} vs stream {tuple(size)}")
+    return size[0], size[1]
 
 
 def fp4_add_rmsnorm(stream: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, out: Fp4Rows, eps: float,
@@ -3251,8 +3251,9 @@ def fp4_product(x: Fp4Rows, w: Fp4Rows, out: torch.Tensor, status: torch.Tensor)
     _check_fp4("fp4_product.x", x)
     _check_fp4("fp4_product.w", w, x.width)
     T, N = x.codes.shape[0], w.codes.shape[0]
-    pitch = out.stride(0) if out.dim() == 2 else 0
-    if not out.is_cuda or out.shape != (T, N) or (N > 1 and out.stride(1) != 1) or (T > 1 and pitch < N):
+    whole = out.is_contiguous()
+    pitch = N if whole else out.stride(0) if out.dim() == 2 else 0
+    if not out.is_cuda or out.shape != (T, N) or not (whole or ((N <= 1 or out.stride(1) == 1) and (T <= 1 or pitch >= N))):
         raise KernelError(f"fp4_product: out {tuple(out.shape)} with strides {out.stride()} on {out.device} for {T} x {N}")
     code = library().q3_fp4_product(x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
                                     T, N, x.width, pitch if pitch > N else N, 1 if dtype_tag(out.dtype) == F32 else 0,

@@ -271,7 +271,9 @@ def test_gated_product_of_what_is_not_finite(rows):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
-@pytest.mark.parametrize("rows,width,inner", [(1, 256, 520), (24, 512, 1000), (300, 264, 328)])
+@pytest.mark.parametrize("rows,width,inner", [(1, 8, 8), (1, 256, 520), (1, 4096, 1200), (3, 4104, 200), (7, 8192 // 2, 328), (24, 512, 1000), (24, 1000, 504),
+                                              (32, 1024, 72), (33, 1024, 72), (4, 8192, 160), (9, 4096, 160), (2, 12288, 64), (2, 100, 80),
+                                              (300, 264, 328)])
 def test_feed_forward_is_its_parts(dtype, rows, width, inner):
     o = ops()
     stream, delta = normal(rows, width, 1).cuda(), (normal(rows, width, 2) * 0.3).to(DT[dtype]).cuda()
@@ -287,12 +289,77 @@ def test_feed_forward_is_its_parts(dtype, rows, width, inner):
     o.fp4_product(a2, down, y2, st)
     assert int(st.item()) == 0
     assert torch.equal(s, s2) and torch.equal(h.codes, h2.codes) and torch.equal(a.codes, a2.codes) and torch.equal(y, y2)
+    for one, other in ((h, h2), (a, a2)):
+        assert torch.equal(plain.read(one.codes, one.scales, one.width)[1], plain.read(other.codes, other.scales, other.width)[1])
     # and against 64 bits: as the last product of what the gate left
     want = plain.read(a.codes, a.scales, inner)[0] @ plain.read(down.codes, down.scales, inner)[0].t()
     tol = product_tolerance(plain.read(a.codes, a.scales, inner)[0], plain.read(down.codes, down.scales, inner)[0])
     assert bool(((y.cpu().double() - want).abs() <= tol + (want.abs() * 2.0 ** -8 if dtype == "bfloat16" else 0)).all())
-    o.fp4_feed_forward(stream, delta, norm, 1e-6, gu, down, h, a, y, st)  # the stream in place
-    assert torch.equal(stream, s) and torch.equal(y, y2)
+    junk = [junk_rows(rows, width), junk_rows(rows, inner)]
+    y.fill_(3)
+    o.fp4_feed_forward(stream.clone(), delta.clone(), norm, 1e-6, gu, down, *junk, delta, st, stream_out=s)  # the output over delta
+    assert torch.equal(delta, y2) and torch.equal(s, s2) and pad_is_zero(junk[0]) and pad_is_zero(junk[1])
+    o.fp4_feed_forward(s, None, norm, 1e-6, gu, down, h, a, y, st, stream_out=stream)  # no delta
+    assert torch.equal(stream, s2) and torch.equal(y, y2)
+
+
+@pytest.mark.parametrize("rows,width", [(1, 256), (24, 512), (40, 512)])
+def test_feed_forward_updates_the_stream_in_place(rows, width):
+    o, inner = ops(), 264
+    stream, delta = normal(rows, width, 1).cuda(), (normal(rows, width, 2) * 0.3).cuda()
+    total = stream + delta
+    norm = torch.ones(width, device="cuda")
+    gu = held(interleaved(normal(inner, width, 4, False), normal(inner, width, 5, False)) * width ** -0.5)[0]
+    down = held(normal(width, inner, 6, False) * inner ** -0.5)[0]
+    h, a, st = o.fp4_rows(rows, width, "cuda"), o.fp4_rows(rows, inner, "cuda"), status()
+    want, y = torch.empty_like(delta), torch.empty_like(delta)
+    o.fp4_feed_forward(total.clone(), None, norm, 1e-6, gu, down, h, a, want, st)
+    o.fp4_feed_forward(stream, delta, norm, 1e-6, gu, down, h, a, y, st)
+    assert torch.equal(stream, total) and torch.equal(y, want) and int(st.item()) == 0
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+def test_feed_forward_right_behind_what_rounds_its_weights(rows):
+    o, width, inner = ops(), 1024, 2000
+    stream, norm = normal(rows, width, 1).cuda(), torch.ones(width, device="cuda")
+    wide = interleaved(normal(inner, width, 4, False), normal(inner, width, 5, False)).cuda()
+    narrow = normal(width, inner, 6, False).cuda()
+    gu, down = o.fp4_rows(2 * inner, width, "cuda"), o.fp4_rows(width, inner, "cuda")
+    h, a, st = o.fp4_rows(rows, width, "cuda"), o.fp4_rows(rows, inner, "cuda"), status()
+    want = y = None
+    for _ in range(4):
+        gu.codes.fill_(0xA5)
+        down.codes.fill_(0xA5)
+        y = torch.empty(rows, width, device="cuda")
+        torch.cuda.synchronize()
+        o.fp4_quantise(narrow, down)
+        o.fp4_quantise(wide, gu)
+        if want is None:
+            torch.cuda.synchronize()
+        o.fp4_feed_forward(stream, None, norm, 1e-6, gu, down, h, a, y, st)
+        want = y if want is None else want
+        assert torch.equal(y, want)
+
+
+def test_feed_forward_gives_up_cleanly():
+    o, rows, width, inner = ops(), 2, 2048, 520
+    stream, norm = normal(rows, width, 1).cuda(), torch.ones(width, device="cuda")
+    gu = held(interleaved(normal(inner, width, 4, False), normal(inner, width, 5, False)))[0]
+    down = held(normal(width, inner, 6, False))[0]
+    h, a, st = o.fp4_rows(rows, width, "cuda"), o.fp4_rows(rows, inner, "cuda"), status()
+    want, y = (torch.empty(rows, width, device="cuda") for _ in range(2))
+    o.fp4_feed_forward(stream, None, norm, 1e-6, gu, down, h, a, want, st)
+    try:
+        o.set_wait_test(limit=1 << 14, drop_copy=0)  # a block may have one stage only
+        o.fp4_feed_forward(stream, None, norm, 1e-6, gu, down, h, a, y, st)
+        torch.cuda.synchronize()
+        word = int(st.item())
+    finally:
+        o.set_wait_test()
+    assert word & 16, f"status {word}: the time-out bit is not set"
+    st.zero_()
+    o.fp4_feed_forward(stream, None, norm, 1e-6, gu, down, h, a, y, st)
+    assert torch.equal(y, want) and int(st.item()) == 0
 
 
 # ---------------------------------------------------------------- calls
