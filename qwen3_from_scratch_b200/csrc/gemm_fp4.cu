@@ -116,21 +116,30 @@ __device__ __forceinline__ void f4_store_rows(const uint32_t (&v0)[32], const ui
     *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = x;
   }
   __syncwarp();
-  const int c = lane & 7, at = col + c * PER;
-  OutT* dst = (OutT*)p.out + (size_t)(row0 + (lane >> 3)) * p.ldc + at;
-  const bool whole = at + PER <= p.N && (((uintptr_t)p.out | (size_t)p.ldc * sizeof(OutT)) & 15) == 0;
+  OutT* dst = (OutT*)p.out + (size_t)row0 * p.ldc + col;
+  const int rows = min(32, p.T - row0);
+  if (col + 8 * PER <= p.N && (((uintptr_t)p.out | (size_t)p.ldc * sizeof(OutT)) & 15) == 0) {  // uniform over the warp
+    const int c = lane & 7;
+    dst += (size_t)(lane >> 3) * p.ldc + c * PER;
 #pragma unroll
-  for (int i = 0; i < 8; ++i, dst += 4 * p.ldc) {
-    const int r = 4 * i + (lane >> 3);
-    const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
-    if (row0 + r < p.T) {
-      if (whole) {
-        *reinterpret_cast<uint4*>(dst) = x;
+    for (int i = 0; i < 8; ++i, dst += 4 * p.ldc) {
+      const int r = 4 * i + (lane >> 3);
+      if (r < rows) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
+    }
+  } else {  // rows off a 16-byte boundary, or the last columns: a word of each row to a lane
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r, dst += p.ldc) {
+      const uint32_t x = *reinterpret_cast<const uint32_t*>(stage + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+      if (EPI == 1) {
+        if (col + lane < p.N) reinterpret_cast<uint32_t*>(dst)[lane] = x;
       } else {
-        const OutT* e = reinterpret_cast<const OutT*>(&x);
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-          if (at + j < p.N) dst[j] = e[j];
+        uint16_t* const two = reinterpret_cast<uint16_t*>(dst) + 2 * lane;
+        if (((uintptr_t)two & 3) == 0 && col + 2 * lane + 1 < p.N) {
+          *reinterpret_cast<uint32_t*>(two) = x;
+        } else {
+          if (col + 2 * lane < p.N) two[0] = (uint16_t)x;
+          if (col + 2 * lane + 1 < p.N) two[1] = (uint16_t)(x >> 16);
+        }
       }
     }
   }
@@ -761,9 +770,9 @@ static int gemm_fp4_few_launch(const CUtensorMap& map_x, const CUtensorMap& map_
 
 // The few-tokens kernel's tiles.  Blocks run one to an SM in rounds; a round takes its stages times what issuing one takes (clocks,
 // measured on one SM: 386, 415 and 470 for 64, 128 and 192 rows of w), and sharing out k costs the sending and adding of sums.
-static F4FewShape f4_few_shape(int T, int N, int K) {
+static F4FewShape f4_few_shape(int T, int N, int K, double* clocks) {
   F4FewShape best{};
-  double best_cost = 0;
+  double best_cost = 0, best_rounds = 0;
   const int sms = sm_count(), k_stages = (fp4_tiles(K) + 1) / 2, rows = T < F4_BM ? T : F4_BM;
   for (int bn = 64; bn <= 192; bn += 64) {
     const long long tiles = (long long)((N + bn - 1) / bn) * ((T + F4_BM - 1) / F4_BM);
@@ -774,6 +783,7 @@ static F4FewShape f4_few_shape(int T, int N, int K) {
       const double cost = rounds * (depth * (bn == 64 ? 386 : bn == 128 ? 415 : 470) + (split > 1 ? 600 + rows * bn / 2 : 0));
       if (best.bn == 0 || cost < best_cost) {
         best_cost = cost;
+        best_rounds = rounds;
         best.bn = bn;
         best.split = split;
         best.depth = depth;
@@ -787,9 +797,11 @@ static F4FewShape f4_few_shape(int T, int N, int K) {
   const int alone = best.split > 1 ? 0 : rows * (best.bn + 4) * 4;  // the sums' place over the ring
   // Up to eight stages a block keeps to half of an SM's shared memory, so that a block of the next kernel fits beside it and has its
   // first stages on their way while this one ends (1 x 4,096 x 12,288, eight stages: 6.2 us in 112 KB, 7.2 in 224); where it works
-  // through more, a deeper ring does more for it (8 x 24,576 x 4,096, sixteen stages: 14.1 us in 112 KB, 12.2 in 160).  All of it
+  // through more and has an SM for itself, a deeper ring does more for it (8 x 24,576 x 4,096, sixteen stages: 14.1 us in 112 KB,
+  // 12.2 in 160).  All of it
   // where that leaves under three stages, or no place for the sums.
-  for (int room = need > 8 ? 160 * 1024 : 112 * 1024;; room = 224 * 1024) {
+  const bool one_each = best_rounds <= 1;
+  for (int room = need > 8 && one_each ? 160 * 1024 : 112 * 1024;; room = 224 * 1024) {
     best.stages = (room - best.received_bytes() - F4_BAR_BYTES) / best.stage_bytes();
     if (best.stages > need) best.stages = need;
     if (best.stages > F4_FEW_MAX_STAGES) best.stages = F4_FEW_MAX_STAGES;
@@ -797,6 +809,9 @@ static F4FewShape f4_few_shape(int T, int N, int K) {
     if (room > 160 * 1024 || ((best.stages >= 3 || best.stages == need) && best.ring_bytes() >= alone)) break;
   }
   while (best.ring_bytes() < alone) ++best.stages;
+  // What it takes, for the choice between the kernels: with many rows a stage takes as long as its bytes do, some 30 a clock.
+  const int issue = best.bn == 64 ? 386 : best.bn == 128 ? 415 : 470, bytes = best.stage_bytes() / 30;
+  *clocks = best_cost + best_rounds * best.depth * (bytes > issue ? bytes - issue : 0);
   return best;
 }
 
@@ -825,10 +840,12 @@ static int f4_pair_slots() {
 // Clocks of the pair kernel's rounds, from measured times: a stage of 192 or 256 columns takes 410 or 522, a tile of 256 a further
 // 1,400.  (192 and 256 columns: 78 and 81 us at 2,048 x 24,576 x 4,096, 44 and 41 at 2,048 x 4,096 x 12,288, 359 and 352 at 8,192 x
 // 5,120 x 25,600.)
-static double f4_pair_cost(int T, int N, int K, int bn) {
+// Rows of results off a 16-byte boundary leave a word of each row to a lane and hold a round up further (3,000 x 9,001 x 2,560:
+// 85 us in float32 and 54 in bfloat16, 53 and 46 with 9,000 columns).
+static double f4_pair_cost(int T, int N, int K, int bn, double stores) {
   const long long tiles = (long long)((N + bn - 1) / bn) * ((T + 255) / 256), slots = f4_pair_slots();
   const int k_stages = (fp4_tiles(K) + 1) / 2;
-  return (double)((tiles + slots - 1) / slots) * (bn == 192 ? k_stages * 410.0 : k_stages * 522.0 + 1400.0);
+  return (double)((tiles + slots - 1) / slots) * (stores + (bn == 192 ? k_stages * 410.0 : k_stages * 522.0 + 1400.0));
 }
 
 template <int EPI, int BN>
@@ -860,12 +877,20 @@ static int gemm_fp4_pair_launch(const void* x_codes, const void* w_codes, const 
 // early: w was not written by the launch before this one.
 template <int EPI>
 static int gemm_fp4(const void* x_codes, const void* w_codes, const F4Args& p, int early, int* status, cudaStream_t stream) {
-  if (p.T > 256 && (long long)((p.T + 255) / 256) * ((p.N + 255) / 256) >= sm_count() / 4) {
-    if (f4_pair_cost(p.T, p.N, p.K, 192) <= f4_pair_cost(p.T, p.N, p.K, 256))
-      return gemm_fp4_pair_launch<EPI, 192>(x_codes, w_codes, p, status, stream);
-    return gemm_fp4_pair_launch<EPI, 256>(x_codes, w_codes, p, status, stream);
+  double few = 0;
+  const F4FewShape shape = f4_few_shape(p.T, p.N, p.K, &few);
+  if (p.T >= F4_BM) {
+    // Pairs of CTAs where their rounds, and some 3,500 clocks that their start and end take longer, are fewer clocks.  Measured, few
+    // / pairs, us: 128 rows 8.1 / 9.2 at 4,096 x 4,096, 17.7 / 16.1 at 24,576 x 4,096; 256 rows 17.8 / 16.5 at 4,096 x 12,288 and
+    // 30.5 / 16.3 at 24,576 x 4,096; 512 rows 4.9 / 6.4 at 1,024 x 1,024, 10.6 / 9.6 at 4,096 x 4,096, 16.7 / 27.3 at 1,000 x 25,600.
+    const bool whole = EPI == 2 || (((uintptr_t)p.out | (size_t)p.ldc * (EPI == 0 ? 2 : 4)) & 15) == 0;
+    const double stores = whole ? 0 : EPI == 0 ? 1700 : 6500;
+    const double narrow = f4_pair_cost(p.T, p.N, p.K, 192, stores), wide = f4_pair_cost(p.T, p.N, p.K, 256, stores);
+    if ((narrow < wide ? narrow : wide) + 3500 < few) {
+      if (narrow <= wide) return gemm_fp4_pair_launch<EPI, 192>(x_codes, w_codes, p, status, stream);
+      return gemm_fp4_pair_launch<EPI, 256>(x_codes, w_codes, p, status, stream);
+    }
   }
-  const F4FewShape shape = f4_few_shape(p.T, p.N, p.K);
   // the maps take two bytes of codes as one bfloat16: only bytes move
   CUtensorMap map_x, map_w;
   const uint64_t cols = fp4_pitch(p.K) / 2;

@@ -154,7 +154,7 @@ def product_tolerance(x, w):
 SIZES = [(1, 1, 1), (1, 8, 31), (1, 127, 32), (1, 130, 33), (2, 129, 64), (3, 64, 65), (7, 300, 127), (8, 128, 128), (9, 16, 129),
          (16, 256, 256), (17, 257, 257), (33, 200, 300), (64, 520, 1000), (65, 100, 2008), (128, 384, 512), (129, 129, 640),
          (200, 1111, 264), (300, 250, 4104), (512, 512, 1024), (700, 777, 776),
-         (257, 4900, 160), (600, 3333, 776), (1030, 2200, 300)]  # the last three by pairs of CTAs
+         (257, 9900, 160), (600, 7000, 776), (128, 20000, 520), (1030, 12200, 300), (1300, 3001, 4104)]  # the last ones by pairs of CTAs
 
 
 @pytest.mark.parametrize("out", list(DT))
@@ -173,7 +173,7 @@ def test_product(out, rows, features, width):
 
 
 @pytest.mark.parametrize("out", list(DT))
-@pytest.mark.parametrize("rows,features", [(1, 290), (40, 290), (300, 290), (520, 3790)])
+@pytest.mark.parametrize("rows,features", [(1, 290), (40, 290), (300, 290), (1040, 7790)])
 @pytest.mark.parametrize("start,more", [(0, 30), (8, 46), (3, 11)])
 def test_product_into_columns(out, rows, features, start, more):
     x, xv = held(normal(rows, 200, rows))
@@ -187,7 +187,7 @@ def test_product_into_columns(out, rows, features, start, more):
     assert bool((wide[:, :start] == 3).all()) and bool((wide[:, end:] == 3).all())
 
 
-@pytest.mark.parametrize("rows,features", [(5, 200), (300, 200), (300, 5000)])
+@pytest.mark.parametrize("rows,features", [(5, 200), (300, 200), (300, 15000)])
 def test_product_rows_beyond_the_first(rows, features):
     """The first rows of a larger buffer whose other rows hold anything, their scales NaN."""
     width = 520
@@ -202,7 +202,7 @@ def test_product_rows_beyond_the_first(rows, features):
     assert bool(((y.cpu().double() - xv @ wv.t()).abs() <= product_tolerance(xv, wv)).all())
 
 
-@pytest.mark.parametrize("rows,features", [(3, 260), (200, 260), (300, 4900)])
+@pytest.mark.parametrize("rows,features", [(3, 260), (200, 260), (300, 19900)])
 def test_product_of_what_is_not_finite(rows, features):
     """A NaN scale reaches the results of its row of x or of w, and no others."""
     xd, wd = normal(rows, 300, 1), normal(features, 300, 2)
@@ -241,8 +241,8 @@ def gated_bounds(xv, wv, act):
 
 @pytest.mark.parametrize("act", ["silu", "relu", "gelu_tanh"])
 @pytest.mark.parametrize("rows,inner,width", [(1, 8, 32), (1, 64, 100), (3, 40, 264), (8, 136, 1024), (24, 200, 520), (33, 504, 256),
-                                              (130, 1000, 384), (300, 320, 600), (513, 600, 512), (300, 2504, 136), (600, 1672, 264),
-                                              (520, 1736, 300)])
+                                              (130, 1000, 384), (300, 320, 600), (513, 600, 512), (300, 7504, 136), (600, 5672, 264),
+                                              (1040, 1736, 1300)])
 def test_gated_product(act, rows, inner, width):
     x, xv = held(normal(rows, width, rows))
     w, wv = held(interleaved(normal(inner, width, 1, False), normal(inner, width, 2, False)) * width ** -0.5)
@@ -363,7 +363,7 @@ def test_feed_forward_gives_up_cleanly():
 
 
 # ---------------------------------------------------------------- calls
-@pytest.mark.parametrize("rows,features", [(4, 600), (333, 600), (333, 4800)])
+@pytest.mark.parametrize("rows,features", [(4, 600), (333, 600), (333, 12800)])
 def test_the_same_inputs_give_the_same_bits_on_any_stream(rows, features):
     x, w = held(normal(rows, 2000, 1))[0], held(normal(features, 2000, 2))[0]
     first = torch.empty(rows, features, device="cuda")
@@ -447,7 +447,7 @@ def test_refusals():
     assert int(st.item()) == 0
 
 
-@pytest.mark.parametrize("rows,features,width", [(3, 200, 3000), (300, 600, 1024), (600, 3400, 1024)])
+@pytest.mark.parametrize("rows,features,width", [(3, 200, 3000), (300, 600, 1024), (1200, 7400, 1024)])
 def test_a_wait_that_runs_out_is_given_up_cleanly(rows, features, width):
     o = ops()
     x, xv = held(normal(rows, width, 1))
