@@ -93,28 +93,26 @@ __device__ __forceinline__ void f4_gate(const float (&g)[N], const float (&u)[N]
   for (int i = 0; i < N; ++i) a[i] = u[i] * __fdividef(g[i], 1.0f + __expf(-slope * g[i] * fmaf(cubic * g[i], g[i], 1.0f)));
 }
 
+// 64 float32 columns as bfloat16, two to a word.
+__device__ __forceinline__ void f4_pack(const uint32_t (&v0)[32], const uint32_t (&v1)[32], uint32_t (&w)[32]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    w[i] = pack2(v0[2 * i], v0[2 * i + 1]);
+    w[16 + i] = pack2(v1[2 * i], v1[2 * i + 1]);
+  }
+}
 // 128 bytes of results (32 float32 or 64 bfloat16 columns from `col` on) of each of the warp's 32 rows, a row to a lane, by way of
 // 4 KB of shared memory: there the lanes change places, so that eight of them store the 128 bytes of a row side by side.  Storing
 // from the accumulator's own order, 16 bytes of 32 different rows at a time, took as long as the main loop (2,048 x 24,576 x
 // 4,096: 90 us with it, 64 without any stores).  16-byte piece c of row r lies at r * 128 + ((c ^ (r % 8)) * 16), off the banks of
 // its neighbours both ways.
 template <int EPI>
-__device__ __forceinline__ void f4_store_rows(const uint32_t (&v0)[32], const uint32_t (&v1)[32], unsigned char* stage, const F4Args& p,
-                                              int row0, int col, int lane) {
+__device__ __forceinline__ void f4_store_rows(const uint32_t (&w)[32], unsigned char* stage, const F4Args& p, int row0, int col, int lane) {
   using OutT = typename std::conditional<EPI == 0, __nv_bfloat16, float>::type;
   constexpr int PER = 16 / sizeof(OutT);  // values of a piece
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    uint4 x;
-    if (EPI == 0) {
-      const uint32_t(&v)[32] = c < 4 ? v0 : v1;
-      const int i = 8 * (c % 4);
-      x = make_uint4(pack2(v[i], v[i + 1]), pack2(v[i + 2], v[i + 3]), pack2(v[i + 4], v[i + 5]), pack2(v[i + 6], v[i + 7]));
-    } else {
-      x = make_uint4(v0[4 * c], v0[4 * c + 1], v0[4 * c + 2], v0[4 * c + 3]);
-    }
-    *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = x;
-  }
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
   __syncwarp();
   OutT* dst = (OutT*)p.out + (size_t)row0 * p.ldc + col;
   const int rows = min(32, p.T - row0);
@@ -491,21 +489,27 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   }
 }
 
-// ---------------------------------------------------------------- many tokens: 256 x 192 or 256 x 256 tiles by pairs of CTAs
+// ---------------------------------------------------------------- many tokens: tiles of 256 x 192, 256 or 384 by pairs of CTAs
 // The CTA of rank r holds rows 128 r .. of the x tile and half of the w tile's rows, rows 128 r .. of the accumulator, its own rows'
-// scales and all of the w tile's scales; the roles are those of gemm_tc_pair_kernel (gemm_tc.cu).  Tensor memory has room for two
-// accumulators of 192 columns beside the scales, and the epilogue of one tile runs under the main loop of the next; of 256
-// columns it has one, whose epilogue takes its columns into registers at once and hands it back, some 1,400 clocks in which the
-// tensor cores stand still.  The wider tile needs less operand traffic for its work and fits some sizes in fewer rounds.
+// scales and all of the w tile's scales; the roles are those of gemm_tc_pair_kernel (gemm_tc.cu).
+//
+// What bounds the main loop is what an SM takes in, 64 bytes a clock: a stage of 192, 256 or 384 columns is 31, 35 or 44 KB and
+// takes the tensor cores 384, 512 or 768 clocks; measured 500, 560 and some 775.  Against that, tensor memory has room for two
+// accumulators only of 192 columns beside the scales, the epilogue of one tile running under the main loop of the next; with one
+// accumulator the tensor cores stand still until the epilogue's warps have it in their registers (of 384 columns, two instructions
+// of 192, as bfloat16: with a gate or float32 results such a tile is not built, 92 us against 79 for 2,048 x 24,576 x 4,096).
 template <int BN, int EPI>
 struct F4Pair {
   static constexpr int ACCS = BN == 192 ? 2 : 1;
+  static constexpr int MMA_N = BN == 384 ? 192 : BN, PARTS = BN / MMA_N;  // columns of an instruction, instructions for a tile's columns
   static constexpr int STORE_BYTES = EPI == 2 ? 0 : 8 * 4096;  // where each of the epilogue's warps turns its rows around
-  static constexpr int STAGES = (BN == 192 ? 7 : 6) - (EPI == 2 ? 0 : 1);
-  static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128, SA_BYTES = 2 * FP4_TILE_BYTES, SB_BYTES = 4 * FP4_TILE_BYTES;
+  static constexpr int STAGES = (BN == 192 ? 7 : BN == 256 ? 6 : 5) - (EPI == 2 ? 0 : 1);
+  static constexpr int W_TILES = BN == 384 ? 3 : 2;  // tiles of scales that a w tile may touch
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128, SA_BYTES = 2 * FP4_TILE_BYTES, SB_BYTES = W_TILES * 2 * FP4_TILE_BYTES;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;
   static constexpr size_t SMEM_BYTES = (size_t)STAGES * STAGE_BYTES + STORE_BYTES + F4_BAR_BYTES;
-  static constexpr uint32_t SCALE_COL = ACCS * BN, COLS = 512;
+  static constexpr uint32_t SCALE_COL = ACCS * BN, SCALE_COLS = 8 + 8 * W_TILES, COLS = 512;  // two sets of scales
+  static_assert(SCALE_COL + 2 * SCALE_COLS <= COLS && (BN != 384 || EPI == 0), "");
 };
 constexpr int F4_PAIR_EPI_WARPS = 8;
 constexpr int F4_PAIR_THREADS = 64 + 32 * F4_PAIR_EPI_WARPS;
@@ -610,7 +614,9 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         const uint32_t bar = cluster_addr(s_addr(&full[s]), 0);
         if (elect_one()) {
           if (rank == 0) mbar_expect_tx(&full[s], 2 * S::STAGE_BYTES);
-          tma_load_2d_pair(b, &map_w, bar, kt * 64, n * BN + (int)rank * (BN / 2));
+#pragma unroll
+          for (int q = 0; q < S::PARTS; ++q)  // of the rows of an instruction the first half is rank 0's
+            tma_load_2d_pair(b + q * (S::MMA_N / 2 * 128), &map_w, bar, kt * 64, n * BN + q * S::MMA_N + (int)rank * (S::MMA_N / 2));
           tma_load_2d_pair(sb, &map_ws, bar, kt * 256, n * BN / FP4_TILE);
           tma_load_2d_pair(sa, &map_xs, bar, kt * 256, m * 2 + (int)rank);
           if ((int)it != tc_drop_copy || rank != 0)  // tests of the give-up path only (see tc_common.cuh)
@@ -644,17 +650,23 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
           const unsigned char *b = a + S::A_BYTES, *sa = b + S::B_BYTES, *sb = sa + S::SA_BYTES;
           const uint64_t a_desc = umma_desc_sw128(a), b_desc = umma_desc_sw128(b), sa_desc = f4_scale_desc(sa), sb_desc = f4_scale_desc(sb);
           // the scales of this stage beside those of the last one, which its instructions may still read
-          const uint32_t ta = tmem + S::SCALE_COL + (it & 1) * 24, tb = ta + 8;
+          const uint32_t ta = tmem + S::SCALE_COL + (it & 1) * S::SCALE_COLS, tb = ta + 8;
           const bool both = across - 2 * kt > 1;
           if (elect_one()) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
               if (h == 0 || both) {
                 f4_copy_scales_pair(ta + 4 * h, sa_desc + h * (FP4_TILE_BYTES >> 4));
-                f4_copy_scales_pair(tb + 8 * h, sb_desc + h * (FP4_TILE_BYTES >> 4));
-                f4_copy_scales_pair(tb + 8 * h + 4, sb_desc + (S::SA_BYTES >> 4) + h * (FP4_TILE_BYTES >> 4));
-                f4_mma_pair(acc, a_desc + 4 * h, b_desc + 4 * h, f4_idesc(BN, 0, 256), ta + 4 * h, tb + shift + 8 * h, (kt | h) != 0);
-                f4_mma_pair(acc, a_desc + 4 * h + 2, b_desc + 4 * h + 2, f4_idesc(BN, 2, 256), ta + 4 * h, tb + shift + 8 * h, 1);
+#pragma unroll
+                for (int j = 0; j < S::W_TILES; ++j)
+                  f4_copy_scales_pair(tb + 4 * (S::W_TILES * h + j), sb_desc + j * (S::SA_BYTES >> 4) + h * (FP4_TILE_BYTES >> 4));
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                  for (int q = 0; q < S::PARTS; ++q)
+                    f4_mma_pair(acc + q * S::MMA_N, a_desc + 4 * h + 2 * e, b_desc + q * (S::MMA_N / 2 * 128 >> 4) + 4 * h + 2 * e,
+                                f4_idesc(S::MMA_N, 2 * e, 256), ta + 4 * h, tb + shift + 4 * S::W_TILES * h + q * (S::MMA_N / 32),
+                                (kt | h | e) != 0);
               }
             umma_commit_pair(&empty[s]);
             if (kt + 1 == k_stages) umma_commit_pair(&acc_full[buf]);
@@ -665,8 +677,9 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
       if (!ok && lane == 0) give_up();
     }
   } else {
-    // two warps for each quarter of the rows: the first 128 columns and the others
-    const int quarter = warp & 3, half = (warp - 2) >> 2, chunks = half ? (BN - 128) / 32 : 4;
+    // two warps for each quarter of the rows, for the first and the other columns
+    constexpr int FIRST = BN == 384 ? 192 : 128;
+    const int quarter = warp & 3, half = (warp - 2) >> 2, pieces = (half ? BN - FIRST : FIRST) / 64;
     unsigned char* const store = smem_raw + (size_t)S::STAGES * S::STAGE_BYTES + (warp - 2) * 4096;  // EPI 0, 1
     uint32_t t = 0;
     for (int tile = pair; tile < num_tiles; tile += pairs, ++t) {
@@ -679,29 +692,53 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         break;
       }
       tcgen05_fence_after();
-      const int row0 = m * 256 + (int)rank * 128 + quarter * 32, n0 = n * BN + half * 128;
-      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN + (uint32_t)half * 128;
-      uint32_t v[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (c < chunks) tmem_ld_32(acc + 32 * c, v[c]);
-      tmem_wait_ld();
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(cluster_addr(s_addr(&acc_empty[buf]), 0));
-      __syncwarp();
-      if (row0 >= p.T) continue;  // uniform over the warp
-#pragma unroll
-      for (int c = 0; c < 4; c += 2) {
-        if (c >= chunks || n0 + 32 * c >= p.N) break;
+      const int row0 = m * 256 + (int)rank * 128 + quarter * 32, n0 = n * BN + half * FIRST;
+      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN + (uint32_t)half * FIRST;
+      auto release = [&]() {
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(cluster_addr(s_addr(&acc_empty[buf]), 0));
+        __syncwarp();
+      };
+      // 64 columns: what leaves
+      auto finish = [&](const uint32_t(&v0)[32], const uint32_t(&v1)[32], int col) {
+        if (row0 >= p.T || col >= p.N) return;  // uniform over the warp
         if (EPI == 2) {
-          if (row0 + lane < p.T) f4_gated_block(v[c], v[c + 1], p, row0 + lane, n0 + 32 * c);
+          if (row0 + lane < p.T) f4_gated_block(v0, v1, p, row0 + lane, col);
+        } else if (EPI == 0) {
+          uint32_t w[32];
+          f4_pack(v0, v1, w);
+          f4_store_rows<EPI>(w, store, p, row0, col, lane);
         } else {
-          f4_store_rows<EPI>(v[c], v[c + 1], store, p, row0, n0 + 32 * c, lane);
-          if (EPI == 1 && n0 + 32 * c + 32 < p.N) f4_store_rows<EPI>(v[c + 1], v[c + 1], store, p, row0, n0 + 32 * c + 32, lane);
+          f4_store_rows<EPI>(v0, store, p, row0, col, lane);
+          if (col + 32 < p.N) f4_store_rows<EPI>(v1, store, p, row0, col + 32, lane);
         }
+      };
+      if (BN != 384) {
+        uint32_t v[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (c < 2 * pieces) tmem_ld_32(acc + 32 * c, v[c]);
+        tmem_wait_ld();
+        release();
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          if (c < pieces) finish(v[2 * c], v[2 * c + 1], n0 + 64 * c);
+      } else {  // bfloat16 results only: a tile of 384 columns fits in the registers as such
+        uint32_t w[3][32];
+#pragma unroll
+        for (int c = 0; c < 3; ++c) {
+          uint32_t v[2][32];
+          tmem_ld_32(acc + 64 * c, v[0]);
+          tmem_ld_32(acc + 64 * c + 32, v[1]);
+          tmem_wait_ld();
+          f4_pack(v[0], v[1], w[c]);
+        }
+        release();
+#pragma unroll
+        for (int c = 0; c < 3; ++c)
+          if (row0 < p.T && n0 + 64 * c < p.N) f4_store_rows<EPI>(w[c], store, p, row0, n0 + 64 * c, lane);
       }
-      __syncwarp();
     }
   }
   tcgen05_fence_before();
@@ -837,15 +874,15 @@ static int f4_pair_slots() {
   return slots[dev];
 }
 
-// Clocks of the pair kernel's rounds, from measured times: a stage of 192 or 256 columns takes 410 or 522, a tile of 256 a further
-// 1,400.  (192 and 256 columns: 78 and 81 us at 2,048 x 24,576 x 4,096, 44 and 41 at 2,048 x 4,096 x 12,288, 359 and 352 at 8,192 x
-// 5,120 x 25,600.)
-// Rows of results off a 16-byte boundary leave a word of each row to a lane and hold a round up further (3,000 x 9,001 x 2,560:
-// 85 us in float32 and 54 in bfloat16, 53 and 46 with 9,000 columns).
-static double f4_pair_cost(int T, int N, int K, int bn, double stores) {
+// Clocks of the pair kernel's rounds: its stages, and what a tile's epilogue holds up.  Measured with 192, 256 and 384 columns, us:
+// 79, 81, 75 at 2,048 x 24,576 x 4,096, 44.5, 41.9, 54.8 at 2,048 x 4,096 x 12,288, 361, 354, 370 at 8,192 x 5,120 x 25,600.  Rows
+// of results off a 16-byte boundary leave a word of each row to a lane and hold a round up further (3,000 x 9,001 x 2,560: 67 us in
+// float32 and 47 in bfloat16, 44 and 35 with 9,000 columns).
+static double f4_pair_cost(int T, int N, int K, int bn, int epi, bool whole) {
   const long long tiles = (long long)((N + bn - 1) / bn) * ((T + 255) / 256), slots = f4_pair_slots();
   const int k_stages = (fp4_tiles(K) + 1) / 2;
-  return (double)((tiles + slots - 1) / slots) * (stores + (bn == 192 ? k_stages * 410.0 : k_stages * 522.0 + 1400.0));
+  const double stage = bn == 192 ? 500 : bn == 256 ? 560 : 775, hold = bn == 192 ? 1000 : bn == 256 ? 2850 : 4800;
+  return (double)((tiles + slots - 1) / slots) * (k_stages * stage + hold + (whole ? 0 : epi == 0 ? 1700 : 6500) * (bn / 192.0));
 }
 
 template <int EPI, int BN>
@@ -861,9 +898,9 @@ static int gemm_fp4_pair_launch(const void* x_codes, const void* w_codes, const 
   CUtensorMap map_x, map_w, map_xs, map_ws;
   const uint64_t cols = fp4_pitch(p.K) / 2, across = fp4_tiles(p.K);
   int code = cached_map(&map_x, x_codes, (uint64_t)p.T, cols, 128);
-  if (!code) code = cached_map(&map_w, w_codes, (uint64_t)p.N, cols, BN / 2);
+  if (!code) code = cached_map(&map_w, w_codes, (uint64_t)p.N, cols, S::MMA_N / 2);
   if (!code) code = f4_scale_map(&map_xs, p.x_scales, fp4_tiles(p.T), across, 1);
-  if (!code) code = f4_scale_map(&map_ws, p.w_scales, fp4_tiles(p.N), across, 2);
+  if (!code) code = f4_scale_map(&map_ws, p.w_scales, fp4_tiles(p.N), across, S::W_TILES);
   if (code) return code;
   const long long tiles = (long long)((p.N + BN - 1) / BN) * ((p.T + 255) / 256);
   if (tiles > 0x3fffffffLL) return Q3_ERR_SIZE;
@@ -874,23 +911,31 @@ static int gemm_fp4_pair_launch(const void* x_codes, const void* w_codes, const 
   return code ? code : last;
 }
 
-// early: w was not written by the launch before this one.
+// early: w was not written by the launch before this one.  form: 0 by the clocks that the forms take, 1 the kernel for a few
+// tokens, 192, 256 or (bfloat16 results) 384 columns by pairs of CTAs.
 template <int EPI>
-static int gemm_fp4(const void* x_codes, const void* w_codes, const F4Args& p, int early, int* status, cudaStream_t stream) {
+static int gemm_fp4(const void* x_codes, const void* w_codes, const F4Args& p, int form, int early, int* status, cudaStream_t stream) {
   double few = 0;
   const F4FewShape shape = f4_few_shape(p.T, p.N, p.K, &few);
-  if (p.T >= F4_BM) {
+  if (form == 0 && p.T >= F4_BM) {
     // Pairs of CTAs where their rounds, and some 3,500 clocks that their start and end take longer, are fewer clocks.  Measured, few
     // / pairs, us: 128 rows 8.1 / 9.2 at 4,096 x 4,096, 17.7 / 16.1 at 24,576 x 4,096; 256 rows 17.8 / 16.5 at 4,096 x 12,288 and
     // 30.5 / 16.3 at 24,576 x 4,096; 512 rows 4.9 / 6.4 at 1,024 x 1,024, 10.6 / 9.6 at 4,096 x 4,096, 16.7 / 27.3 at 1,000 x 25,600.
     const bool whole = EPI == 2 || (((uintptr_t)p.out | (size_t)p.ldc * (EPI == 0 ? 2 : 4)) & 15) == 0;
-    const double stores = whole ? 0 : EPI == 0 ? 1700 : 6500;
-    const double narrow = f4_pair_cost(p.T, p.N, p.K, 192, stores), wide = f4_pair_cost(p.T, p.N, p.K, 256, stores);
-    if ((narrow < wide ? narrow : wide) + 3500 < few) {
-      if (narrow <= wide) return gemm_fp4_pair_launch<EPI, 192>(x_codes, w_codes, p, status, stream);
-      return gemm_fp4_pair_launch<EPI, 256>(x_codes, w_codes, p, status, stream);
+    double clocks = few - 3500;
+    for (int bn : {192, 256, 384}) {
+      if (bn == 384 && EPI != 0) break;
+      const double c = f4_pair_cost(p.T, p.N, p.K, bn, EPI, whole);
+      if (c < clocks) {
+        clocks = c;
+        form = bn;
+      }
     }
   }
+  if (form == 192) return gemm_fp4_pair_launch<EPI, 192>(x_codes, w_codes, p, status, stream);
+  if (form == 256) return gemm_fp4_pair_launch<EPI, 256>(x_codes, w_codes, p, status, stream);
+  if (form == 384) return EPI == 0 ? gemm_fp4_pair_launch<EPI, EPI == 0 ? 384 : 256>(x_codes, w_codes, p, status, stream) : Q3_ERR_SIZE;
+  if (form != 0 && form != 1) return Q3_ERR_SIZE;
   // the maps take two bytes of codes as one bfloat16: only bytes move
   CUtensorMap map_x, map_w;
   const uint64_t cols = fp4_pitch(p.K) / 2;
@@ -907,22 +952,22 @@ static bool f4_aligned(const void* a, const void* b, const void* c, const void* 
 }
 
 static int fp4_product(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out, int T, int N,
-                       int K, long long ldc, int out_f32, int early, int* status, cudaStream_t stream) {
+                       int K, long long ldc, int out_f32, int form, int early, int* status, cudaStream_t stream) {
   if (T <= 0) return 0;
   if (!f4_sizes_ok(T, N, K) || ldc < N) return Q3_ERR_SIZE;
   if (!f4_aligned(x_codes, x_scales, w_codes, w_scales)) return Q3_ERR_ALIGN;
   const F4Args p{(const uint8_t*)x_scales, (const uint8_t*)w_scales, out, ldc, nullptr, nullptr, T, N, K, 0};
-  if (out_f32) return gemm_fp4<1>(x_codes, w_codes, p, early, status, stream);
-  return gemm_fp4<0>(x_codes, w_codes, p, early, status, stream);
+  if (out_f32) return gemm_fp4<1>(x_codes, w_codes, p, form, early, status, stream);
+  return gemm_fp4<0>(x_codes, w_codes, p, form, early, status, stream);
 }
 
 static int fp4_gated_product(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out_codes,
-                             void* out_scales, int T, int N, int K, int act, int early, int* status, cudaStream_t stream) {
+                             void* out_scales, int T, int N, int K, int act, int form, int early, int* status, cudaStream_t stream) {
   if (T <= 0) return 0;
   if (!f4_sizes_ok(T, N, K) || N % 16 || (act != Q3_ACT_SILU && act != Q3_ACT_RELU && act != Q3_ACT_GELU_TANH)) return Q3_ERR_SIZE;
   if (!f4_aligned(x_codes, x_scales, w_codes, w_scales) || !f4_aligned(out_codes, out_scales, nullptr, nullptr)) return Q3_ERR_ALIGN;
   const F4Args p{(const uint8_t*)x_scales, (const uint8_t*)w_scales, nullptr, 0, (uint8_t*)out_codes, (uint8_t*)out_scales, T, N, K, act};
-  return gemm_fp4<2>(x_codes, w_codes, p, early, status, stream);
+  return gemm_fp4<2>(x_codes, w_codes, p, form, early, status, stream);
 }
 
 }  // namespace q3
@@ -930,18 +975,18 @@ static int fp4_gated_product(const void* x_codes, const void* x_scales, const vo
 extern "C" int q3_fp4_add_rmsnorm(const float* in, const void* delta, int dtype, const float* w, float* out, void* codes,
                                   void* scales, int R, int H, float eps, cudaStream_t stream);
 
-// out[T, N] (row pitch ldc) = x w^T of rows held in four bits; out_f32: float32 results, else bfloat16.
+// out[T, N] (row pitch ldc) = x w^T of rows held in four bits; out_f32: float32 results, else bfloat16.  form: see gemm_fp4.
 extern "C" int q3_fp4_product(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out, int T,
-                              int N, int K, long long ldc, int out_f32, int* status, cudaStream_t stream) {
-  return q3::fp4_product(x_codes, x_scales, w_codes, w_scales, out, T, N, K, ldc, out_f32, q3::last_launch_was_plain(stream), status,
+                              int N, int K, long long ldc, int out_f32, int form, int* status, cudaStream_t stream) {
+  return q3::fp4_product(x_codes, x_scales, w_codes, w_scales, out, T, N, K, ldc, out_f32, form, q3::last_launch_was_plain(stream), status,
                          stream);
 }
 
 // act(gate) * up as rows held in four bits: w's N = 2 I rows alternate gate/up in blocks of eight, the output has T rows of I.
 extern "C" int q3_fp4_gated_product(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales,
-                                    void* out_codes, void* out_scales, int T, int N, int K, int act, int* status,
+                                    void* out_codes, void* out_scales, int T, int N, int K, int act, int form, int* status,
                                     cudaStream_t stream) {
-  const int code = q3::fp4_gated_product(x_codes, x_scales, w_codes, w_scales, out_codes, out_scales, T, N, K, act,
+  const int code = q3::fp4_gated_product(x_codes, x_scales, w_codes, w_scales, out_codes, out_scales, T, N, K, act, form,
                                          q3::last_launch_was_plain(stream), status, stream);
   q3::note_stream_written();  // rows that a product after it might take as its w
   return code;
@@ -955,9 +1000,9 @@ extern "C" int q3_fp4_feed_forward(const float* stream_in, const void* delta, co
   int code = q3_fp4_add_rmsnorm(stream_in, delta, dtype, norm, stream_out, h_codes, h_scales, T, H, eps, stream);
   if (code) return code;
   // neither product's w was written by the launch before it, which is the one above it here
-  code = q3::fp4_gated_product(h_codes, h_scales, gu_codes, gu_scales, a_codes, a_scales, T, 2 * I, H, act, 1, status, stream);
+  code = q3::fp4_gated_product(h_codes, h_scales, gu_codes, gu_scales, a_codes, a_scales, T, 2 * I, H, act, 0, 1, status, stream);
   if (code) return code;
-  return q3::fp4_product(a_codes, a_scales, down_codes, down_scales, y, T, H, I, H, dtype == Q3_F32, 1, status, stream);
+  return q3::fp4_product(a_codes, a_scales, down_codes, down_scales, y, T, H, I, H, dtype == Q3_F32, 0, 1, status, stream);
 }
 
 // For the tests of the give-up path: see set_wait_test in tc_common.cuh.

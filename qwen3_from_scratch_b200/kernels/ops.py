@@ -82,10 +82,10 @@ _SIGNATURES = {
     "q3_fp4_quantise": [_c_void_p, _c_int, _c_ll, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p],
     "q3_fp4_add_rmsnorm": [_c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_float,
                            _c_void_p],
-    "q3_fp4_product": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_ll, _c_int, _c_void_p,
-                       _c_void_p],
+    "q3_fp4_product": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_ll, _c_int, _c_int,
+                       _c_void_p, _c_void_p],
     "q3_fp4_gated_product": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int,
-                             _c_void_p, _c_void_p],
+                             _c_int, _c_void_p, _c_void_p],
     "q3_fp4_feed_forward": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_float, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                             _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
                             _c_void_p, _c_void_p],
@@ -3245,9 +3245,13 @@ def fp4_add_rmsnorm(stream: torch.Tensor, delta: Optional[torch.Tensor], weight:
     _done("fp4_add_rmsnorm", code, f"width {H}")
 
 
-def fp4_product(x: Fp4Rows, w: Fp4Rows, out: torch.Tensor, status: torch.Tensor) -> None:
+FP4_FORMS = {None: 0, "few": 1, "pair192": 192, "pair256": 256, "pair384": 384}
+
+
+def fp4_product(x: Fp4Rows, w: Fp4Rows, out: torch.Tensor, status: torch.Tensor, form: Optional[str] = None) -> None:
     """out[T, N] = x[T, K] @ w[N, K]^T of rows held in four bits, accumulated in float32; out bfloat16 or float32, also a column
-    view of a wider buffer."""
+    view of a wider buffer.  ``form``: one of ``FP4_FORMS`` instead of the one that the sizes ask for (a few tokens' small tiles,
+    or tiles of that many columns by pairs of CTAs, 384 for bfloat16 results only)."""
     _check_fp4("fp4_product.x", x)
     _check_fp4("fp4_product.w", w, x.width)
     T, N = x.codes.shape[0], w.codes.shape[0]
@@ -3257,7 +3261,7 @@ def fp4_product(x: Fp4Rows, w: Fp4Rows, out: torch.Tensor, status: torch.Tensor)
         raise KernelError(f"fp4_product: out {tuple(out.shape)} with strides {out.stride()} on {out.device} for {T} x {N}")
     code = library().q3_fp4_product(x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
                                     T, N, x.width, pitch if pitch > N else N, 1 if dtype_tag(out.dtype) == F32 else 0,
-                                    status.data_ptr(), _stream())
+                                    FP4_FORMS[form], status.data_ptr(), _stream())
     if code:
         _done("fp4_product", code, f"T {T} N {N} K {x.width}")
 
@@ -3268,15 +3272,17 @@ def _fp4_gate(name: str, activation: str) -> int:
     return activation_code(activation, gate=True)
 
 
-def fp4_gated_product(x: Fp4Rows, w: Fp4Rows, out: Fp4Rows, status: torch.Tensor, activation: str = "silu") -> None:
+def fp4_gated_product(x: Fp4Rows, w: Fp4Rows, out: Fp4Rows, status: torch.Tensor, activation: str = "silu",
+                      form: Optional[str] = None) -> None:
     """out = the rows of act(gate) * up, rounded as by ``fp4_quantise`` from float32: w's 2 I rows alternate gate/up in blocks
-    of eight (I a multiple of 8), gate and up are the products of x with them."""
+    of eight (I a multiple of 8), gate and up are the products of x with them.  ``form``: see ``fp4_product``."""
     _check_fp4("fp4_gated_product.x", x)
     _check_fp4("fp4_gated_product.w", w, x.width)
     _check_fp4("fp4_gated_product.out", out, w.rows // 2, x.rows)
     code = library().q3_fp4_gated_product(x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(),
                                           out.codes.data_ptr(), out.scales.data_ptr(), x.rows, w.rows, x.width,
-                                          _fp4_gate("fp4_gated_product", activation), status.data_ptr(), _stream())
+                                          _fp4_gate("fp4_gated_product", activation), FP4_FORMS[form], status.data_ptr(),
+                                          _stream())
     _done("fp4_gated_product", code, f"T {x.rows} N {w.rows} K {x.width}")
 
 
