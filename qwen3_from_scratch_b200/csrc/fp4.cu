@@ -234,12 +234,17 @@ static int fp4_quantise_launch(const void* x, long long x_pitch, uint8_t* codes,
     q3::launch(fp4_quantise_kernel<T, true, V>, grid, dim3(256), 0, stream, (const T*)x, x_pitch, codes, scales, (V*)values, full, R, K);
   else
     q3::launch(fp4_quantise_kernel<T, false, V>, grid, dim3(256), 0, stream, (const T*)x, x_pitch, codes, scales, (V*)values, full, R, K);
-  note_stream_written();  // a product after it may take these rows as its w, which it reads ahead of its wait
   return launch_status();
 }
 
+// ---------------------------------------------------------------- behind an RMSNorm
 // One block per row: s = stream + delta goes to stream_out, s / sqrt(mean(s^2) + eps) * w is rounded.  A thread keeps its
 // eight values of every `8 blockDim` of the row in registers between the sum and the rounding.  stream_out may be stream_in.
+// What bounds it is memory, with the sum of each block in between (2,048 x 4,096, bfloat16 delta: 18 us for 88 MB, 4.9 TB/s, four
+// blocks to an SM hiding each other's sums; blocks that go from row to row and ask for the next one ahead of the sum took 23, the
+// registers for it leaving fewer of them), and for few rows the latency of its chain (1 x 4,096: 3.3 to 4 us between two launches).
+// The weight is read behind the wait like the rest: ahead of it gained nothing that could be measured over the three launches
+// of a feed-forward.
 constexpr int FP4_NORM_MAX = 1024 * 8 * 4;
 template <typename T, int G>
 __global__ void __launch_bounds__(1024)
@@ -253,12 +258,12 @@ fp4_add_rmsnorm_kernel(const float* stream_in, const T* __restrict__ delta, cons
     if (vec) fp4_load_row8<float, true>(w, col, H, wv[g]);
     else fp4_load_row8<float, false>(w, col, H, wv[g]);
   };
-  constexpr bool AHEAD = G <= 2;  // no kernel writes the weight: it is read ahead of the wait where the registers suffice
+  pdl_wait();
+  pdl_launch_dependents();
+  constexpr bool AHEAD = G <= 2;  // where the registers suffice
 #pragma unroll
   for (int g = 0; g < G; ++g)
     if (AHEAD) load_weight(g);
-  pdl_wait();
-  pdl_launch_dependents();
   const size_t r = blockIdx.x;
   const float* in = stream_in + r * H;
   float v[G][8];
@@ -316,7 +321,7 @@ static int fp4_add_rmsnorm_launch(const float* in, const void* delta, const floa
   else if (g == 2) Q3_NORM(2);
   else Q3_NORM(4);
 #undef Q3_NORM
-  note_stream_written();  // the stream, and rows that a product might take as its w
+  note_stream_written();
   return launch_status();
 }
 

@@ -4,17 +4,16 @@
 // the gate is applied and each 32 results are rounded to the same format, so that the [T, 2 I] product never goes to memory.
 //
 // Both kernels have the same three roles:
-//   warp 0  brings the codes of 256 values of k at a time (128 bytes of each row) into shared memory by TMA
-//                        with the 128-byte swizzle, and their scales in whole 512-byte tiles;
-//   warp 1  copies each tile of scales into tensor memory (tcgen05.cp, in order with the instructions of the
-//                        same thread before and behind it) and issues four instructions of k = 64 per stage;
-//   the other warps      the epilogue.
+//   warp 0           brings the codes of 256 values of k at a time (128 bytes of each row) into shared memory by TMA with the
+//                    128-byte swizzle, and their scales in whole 512-byte tiles;
+//   warp 1           copies each tile of scales into tensor memory (tcgen05.cp, in order with the instructions of the same
+//                    thread before and behind it) and issues instructions of k = 64, four for a stage's columns;
+//   the other warps  the epilogue.
 // An instruction reads a row's scales of k = 64 from two of the four bytes of a tensor-memory column; which two is in its
 // descriptor.  Every wait on an mbarrier is bounded, as in gemm_tc.cu.
 //
-// gemm_fp4_few_kernel: 128 x 128 tiles and, where the tiles are fewer than the blocks that the SMs hold, several blocks per
-// tile that share out the range of k and add their sums up through each other's shared memory (a cluster).
-// gemm_fp4_pair_kernel: 256 x 256 tiles by pairs of CTAs, for many tokens.
+// gemm_fp4_few_kernel: small tiles; where they are fewer than the SMs, several blocks per tile share out the range of k.
+// gemm_fp4_pair_kernel: tiles of 256 rows by pairs of CTAs, for many tokens.
 #include "fp4.cuh"
 #include "tc_common.cuh"
 
@@ -179,15 +178,16 @@ __device__ __forceinline__ void f4_gated_block(const uint32_t (&v0)[32], const u
 
 // ---------------------------------------------------------------- a few tokens: small tiles, k shared out
 // A tile is up to 128 rows of x by 64, 128 or 192 rows of w, and `split` blocks of a cluster share out its range of k.  What
-// bounds it is w's bytes where w is large and the chain of latencies between two kernels where it is not, so the sizes are chosen
-// (f4_few_shape) to give each SM one block that leaves room for a block of the next kernel, which then has its first stages of w
-// on their way while this one works.
+// bounds it is w's bytes where w is large (8 x 24,576 x 4,096: 12.4 us, 4.3 TB/s between the start of one call and of the next, some
+// 5.7 while w streams) and the chain of latencies between two kernels where it is not (64 x 4,096 x 4,096: 6.2 us for 1.5 us of
+// bytes: 1 from the kernel before to this one's start, 1 for x, 1 for the main loop, 2 for the sums and the results), so the sizes
+// are chosen (f4_few_shape) to give each SM one block.
 //
 // The blocks of a cluster send each row of sums, by asynchronous stores that the receiver's mbarrier counts, to the block that
 // finishes that row (rank r % split).  No block reads another's memory, so none has to stay for the others: a barrier of the
-// whole cluster behind the reading took 1.1 us, as long as a stage of the main loop takes three times over.
+// whole cluster behind the reading took 1.1 us.  The stores take some two clocks per 16 bytes, so many rows are not shared out.
 constexpr int F4_FEW_THREADS = 192;
-constexpr int F4_BAR_BYTES = 512;
+constexpr int F4_BAR_BYTES = 512;  // barriers and the address of the tensor memory, in both kernels
 constexpr int F4_FEW_MAX_STAGES = 24;
 constexpr int F4_FEW_MAX_SPLIT = 8;
 constexpr int F4_FEW_COLS = 256;  // tensor memory: up to 192 columns of sums, two times 24 of scales
@@ -202,8 +202,8 @@ struct F4FewShape {
   __host__ __device__ int b_bytes() const { return bn * 128; }
   __host__ __device__ int w_scale_tiles() const { return (bn + FP4_TILE - 1) / FP4_TILE; }
   __host__ __device__ int stage_bytes() const { return a_bytes() + b_bytes() + (1 + w_scale_tiles()) * 2 * FP4_TILE_BYTES; }
-  // the last stage's x tile is read as 128 rows
-  __host__ __device__ int ring_bytes() const { return stages * stage_bytes() + (128 * 128 > stage_bytes() ? 128 * 128 - stage_bytes() : 0); }
+  __host__ __device__ int behind_bytes() const { return 128 * 128 > stage_bytes() ? 128 * 128 - stage_bytes() : 0; }  // the last x tile is read as 128 rows
+  __host__ __device__ int ring_bytes() const { return stages * stage_bytes() + behind_bytes(); }
   __host__ __device__ int received_bytes() const { return split > 1 ? split * slots * bn * 4 : 0; }
   __host__ __device__ size_t smem_bytes() const { return (size_t)ring_bytes() + received_bytes() + F4_BAR_BYTES; }
 };
@@ -278,7 +278,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for before anything is sent
 
   if (warp == 0) {
-    // Where the launch before this one did not write w, its part of the ring's first round goes out ahead of the wait.
+    // Where w is known not to come from the kernel before, its part of the ring's first round goes out ahead of the wait.
     const int ahead = early ? min(stages, k_count) : 0;
     if (aligned && elect_one()) {
       tma_prefetch_map(&map_x);
@@ -746,6 +746,8 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
   cluster_sync_all();
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
 }
+
+// ---------------------------------------------------------------- launches
 // A launch with blocks in clusters of `cluster` along x.
 template <typename... KArgs, typename... Args>
 static int f4_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream, Args... args) {
@@ -830,20 +832,17 @@ static F4FewShape f4_few_shape(int T, int N, int K, double* clocks) {
   best.a_rows = (rows + 7) / 8 * 8;
   best.slots = (rows + best.split - 1) / best.split;
   best.split_inverse = (65536 + best.split - 1) / best.split;
-  const int need = best.depth;
   const int alone = best.split > 1 ? 0 : rows * (best.bn + 4) * 4;  // the sums' place over the ring
-  // Up to eight stages a block keeps to half of an SM's shared memory, so that a block of the next kernel fits beside it and has its
-  // first stages on their way while this one ends (1 x 4,096 x 12,288, eight stages: 6.2 us in 112 KB, 7.2 in 224); where it works
-  // through more and has an SM for itself, a deeper ring does more for it (8 x 24,576 x 4,096, sixteen stages: 14.1 us in 112 KB,
-  // 12.2 in 160).  All of it
+  // Up to eight stages a block keeps to half of an SM's shared memory, so that a block of the next kernel fits beside it and starts
+  // while this one ends (1 x 4,096 x 12,288, eight stages: 6.2 us in 112 KB, 7.2 in 224); where it works through more and has an
+  // SM for itself, a deeper ring does more for it (8 x 24,576 x 4,096, sixteen stages: 14.1 us in 112 KB, 12.4 in 160).  All of it
   // where that leaves under three stages, or no place for the sums.
-  const bool one_each = best_rounds <= 1;
-  for (int room = need > 8 && one_each ? 160 * 1024 : 112 * 1024;; room = 224 * 1024) {
-    best.stages = (room - best.received_bytes() - F4_BAR_BYTES) / best.stage_bytes();
-    if (best.stages > need) best.stages = need;
+  for (int room = best.depth > 8 && best_rounds <= 1 ? 160 * 1024 : 112 * 1024;; room = 224 * 1024) {
+    best.stages = (room - best.behind_bytes() - best.received_bytes() - F4_BAR_BYTES) / best.stage_bytes();
+    if (best.stages > best.depth) best.stages = best.depth;
     if (best.stages > F4_FEW_MAX_STAGES) best.stages = F4_FEW_MAX_STAGES;
     if (best.stages < 1) best.stages = 1;
-    if (room > 160 * 1024 || ((best.stages >= 3 || best.stages == need) && best.ring_bytes() >= alone)) break;
+    if (room > 160 * 1024 || ((best.stages >= 3 || best.stages == best.depth) && best.ring_bytes() >= alone)) break;
   }
   while (best.ring_bytes() < alone) ++best.stages;
   // What it takes, for the choice between the kernels: with many rows a stage takes as long as its bytes do, some 30 a clock.
@@ -911,7 +910,7 @@ static int gemm_fp4_pair_launch(const void* x_codes, const void* w_codes, const 
   return code ? code : last;
 }
 
-// early: w was not written by the launch before this one.  form: 0 by the clocks that the forms take, 1 the kernel for a few
+// early: w was not written by the kernel that runs before this one.  form: 0 by the clocks that the forms take, 1 the kernel for a few
 // tokens, 192, 256 or (bfloat16 results) 384 columns by pairs of CTAs.
 template <int EPI>
 static int gemm_fp4(const void* x_codes, const void* w_codes, const F4Args& p, int form, int early, int* status, cudaStream_t stream) {
@@ -978,28 +977,26 @@ extern "C" int q3_fp4_add_rmsnorm(const float* in, const void* delta, int dtype,
 // out[T, N] (row pitch ldc) = x w^T of rows held in four bits; out_f32: float32 results, else bfloat16.  form: see gemm_fp4.
 extern "C" int q3_fp4_product(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out, int T,
                               int N, int K, long long ldc, int out_f32, int form, int* status, cudaStream_t stream) {
-  return q3::fp4_product(x_codes, x_scales, w_codes, w_scales, out, T, N, K, ldc, out_f32, form, q3::last_launch_was_plain(stream), status,
-                         stream);
+  return q3::fp4_product(x_codes, x_scales, w_codes, w_scales, out, T, N, K, ldc, out_f32, form, 0, status, stream);
 }
 
 // act(gate) * up as rows held in four bits: w's N = 2 I rows alternate gate/up in blocks of eight, the output has T rows of I.
 extern "C" int q3_fp4_gated_product(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales,
                                     void* out_codes, void* out_scales, int T, int N, int K, int act, int form, int* status,
                                     cudaStream_t stream) {
-  const int code = q3::fp4_gated_product(x_codes, x_scales, w_codes, w_scales, out_codes, out_scales, T, N, K, act, form,
-                                         q3::last_launch_was_plain(stream), status, stream);
-  q3::note_stream_written();  // rows that a product after it might take as its w
-  return code;
+  return q3::fp4_gated_product(x_codes, x_scales, w_codes, w_scales, out_codes, out_scales, T, N, K, act, form, 0, status, stream);
 }
 
-// A gated feed-forward behind its norm, in three launches: the norm's rows into h, the gated product into a, y = a w_down^T.
+// A gated feed-forward behind its norm, in three launches: the norm's rows into h, the gated product into a, y = a w_down^T.  What
+// runs before each product is the launch above it here, which writes neither product's w, so both may read theirs ahead of it; all
+// that ran before this call is over when the norm's kernel lets the next one start.  (Before a product called by itself anything
+// may have run, the kernel that writes its w included; there reading ahead gains nothing that could be measured.)
 extern "C" int q3_fp4_feed_forward(const float* stream_in, const void* delta, const float* norm, float* stream_out, float eps,
                                    const void* gu_codes, const void* gu_scales, const void* down_codes, const void* down_scales,
                                    void* h_codes, void* h_scales, void* a_codes, void* a_scales, void* y, int dtype, int T,
                                    int H, int I, int act, int* status, cudaStream_t stream) {
   int code = q3_fp4_add_rmsnorm(stream_in, delta, dtype, norm, stream_out, h_codes, h_scales, T, H, eps, stream);
   if (code) return code;
-  // neither product's w was written by the launch before it, which is the one above it here
   code = q3::fp4_gated_product(h_codes, h_scales, gu_codes, gu_scales, a_codes, a_scales, T, 2 * I, H, act, 0, 1, status, stream);
   if (code) return code;
   return q3::fp4_product(a_codes, a_scales, down_codes, down_scales, y, T, H, I, H, dtype == Q3_F32, 0, 1, status, stream);
