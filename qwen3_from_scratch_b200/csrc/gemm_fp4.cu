@@ -494,10 +494,12 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 // scales and all of the w tile's scales; the roles are those of gemm_tc_pair_kernel (gemm_tc.cu).
 //
 // What bounds the main loop is what an SM takes in, 64 bytes a clock: a stage of 192, 256 or 384 columns is 31, 35 or 44 KB and
-// takes the tensor cores 384, 512 or 768 clocks; measured 500, 560 and some 775.  Against that, tensor memory has room for two
+// takes the tensor cores 384, 512 or 768 clocks; measured 490, 522 and 800.  Against that, tensor memory has room for two
 // accumulators only of 192 columns beside the scales, the epilogue of one tile running under the main loop of the next; with one
-// accumulator the tensor cores stand still until the epilogue's warps have it in their registers (of 384 columns, two instructions
-// of 192, as bfloat16: with a gate or float32 results such a tile is not built, 92 us against 79 for 2,048 x 24,576 x 4,096).
+// accumulator the tensor cores stand still until the epilogue's warps have it in their registers, which takes 450 clocks, and some
+// 1,000 with the ways there and back (of 384 columns, two instructions of 192, as bfloat16: with a gate or float32 results, which
+// the registers do not hold, such a tile took 92 us against 79 for 2,048 x 24,576 x 4,096 and is not built).  For long calls the
+// device holds its 1 kW by its clock, at about 1.6 GHz: 2,048 x 24,576 x 4,096 one after another 86 us, 73 with pauses.
 template <int BN, int EPI>
 struct F4Pair {
   static constexpr int ACCS = BN == 192 ? 2 : 1;
@@ -526,6 +528,14 @@ __device__ __forceinline__ void f4_mma_pair(uint32_t d, uint64_t a, uint64_t b, 
 // Each CTA of the pair copies from its own shared memory, at this place, into its own tensor memory.
 __device__ __forceinline__ void f4_copy_scales_pair(uint32_t tmem, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+
+// An arrival on a barrier of the pair that orders nothing by itself: what goes before it (a warp's reads of tensor memory) and behind
+// the wait for it (instructions that write there) is ordered by the tcgen05 fences on either side.  One that releases at the
+// cluster's scope waits for the warp's stores to memory: 1,050 to 3,600 clocks of every tile, 81 us instead of 74 for 2,048 x 24,576
+// x 4,096 in tiles of 256 columns.
+__device__ __forceinline__ void f4_arrive_relaxed(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
 // Tile number `i` of a walk over m_tiles x n_tiles in which GROUP tiles of x stay in the second-level cache.
@@ -697,7 +707,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
       auto release = [&]() {
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(cluster_addr(s_addr(&acc_empty[buf]), 0));
+        if (lane == 0) f4_arrive_relaxed(cluster_addr(s_addr(&acc_empty[buf]), 0));
         __syncwarp();
       };
       // 64 columns: what leaves
@@ -725,16 +735,20 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         for (int c = 0; c < 2; ++c)
           if (c < pieces) finish(v[2 * c], v[2 * c + 1], n0 + 64 * c);
       } else {  // bfloat16 results only: a tile of 384 columns fits in the registers as such
-        uint32_t w[3][32];
+        uint32_t v[2][2][32], w[3][32];
+        tmem_ld_32(acc, v[0][0]);
+        tmem_ld_32(acc + 32, v[0][1]);
 #pragma unroll
-        for (int c = 0; c < 3; ++c) {
-          uint32_t v[2][32];
-          tmem_ld_32(acc + 64 * c, v[0]);
-          tmem_ld_32(acc + 64 * c + 32, v[1]);
+        for (int c = 0; c < 3; ++c) {  // the next 64 columns on their way while these are packed
           tmem_wait_ld();
-          f4_pack(v[0], v[1], w[c]);
+          if (c < 2) {
+            tmem_ld_32(acc + 64 * (c + 1), v[(c + 1) & 1][0]);
+            tmem_ld_32(acc + 64 * (c + 1) + 32, v[(c + 1) & 1][1]);
+          } else {
+            release();
+          }
+          f4_pack(v[c & 1][0], v[c & 1][1], w[c]);
         }
-        release();
 #pragma unroll
         for (int c = 0; c < 3; ++c)
           if (row0 < p.T && n0 + 64 * c < p.N) f4_store_rows<EPI>(w[c], store, p, row0, n0 + 64 * c, lane);
@@ -873,14 +887,15 @@ static int f4_pair_slots() {
   return slots[dev];
 }
 
-// Clocks of the pair kernel's rounds: its stages, and what a tile's epilogue holds up.  Measured with 192, 256 and 384 columns, us:
-// 79, 81, 75 at 2,048 x 24,576 x 4,096, 44.5, 41.9, 54.8 at 2,048 x 4,096 x 12,288, 361, 354, 370 at 8,192 x 5,120 x 25,600.  Rows
+// Clocks of the pair kernel's rounds: its stages, and what a tile takes beside them.  Measured with 192, 256 and 384 columns, us:
+// 79, 77, 73 at 2,048 x 24,576 x 4,096, 43, 40, 53 at 2,048 x 4,096 x 12,288, 350, 341, 364 at 8,192 x 5,120 x 25,600, 16.4, 20,
+// 28 at 256 x 4,096 x 12,288 (a stage 420, 560 and 715 clocks, and 1,700, 1,200 and 3,700 a tile, fit these and ten more).  Rows
 // of results off a 16-byte boundary leave a word of each row to a lane and hold a round up further (3,000 x 9,001 x 2,560: 67 us in
 // float32 and 47 in bfloat16, 44 and 35 with 9,000 columns).
 static double f4_pair_cost(int T, int N, int K, int bn, int epi, bool whole) {
   const long long tiles = (long long)((N + bn - 1) / bn) * ((T + 255) / 256), slots = f4_pair_slots();
   const int k_stages = (fp4_tiles(K) + 1) / 2;
-  const double stage = bn == 192 ? 500 : bn == 256 ? 560 : 775, hold = bn == 192 ? 1000 : bn == 256 ? 2850 : 4800;
+  const double stage = bn == 192 ? 420 : bn == 256 ? 560 : 715, hold = bn == 192 ? 1700 : bn == 256 ? 1200 : 3700;
   return (double)((tiles + slots - 1) / slots) * (k_stages * stage + hold + (whole ? 0 : epi == 0 ? 1700 : 6500) * (bn / 192.0));
 }
 
@@ -918,8 +933,8 @@ static int gemm_fp4(const void* x_codes, const void* w_codes, const F4Args& p, i
   const F4FewShape shape = f4_few_shape(p.T, p.N, p.K, &few);
   if (form == 0 && p.T >= F4_BM) {
     // Pairs of CTAs where their rounds, and some 3,500 clocks that their start and end take longer, are fewer clocks.  Measured, few
-    // / pairs, us: 128 rows 8.1 / 9.2 at 4,096 x 4,096, 17.7 / 16.1 at 24,576 x 4,096; 256 rows 17.8 / 16.5 at 4,096 x 12,288 and
-    // 30.5 / 16.3 at 24,576 x 4,096; 512 rows 4.9 / 6.4 at 1,024 x 1,024, 10.6 / 9.6 at 4,096 x 4,096, 16.7 / 27.3 at 1,000 x 25,600.
+    // / pairs, us: 128 rows 9.0 / 8.4 at 4,096 x 4,096, 18.3 / 16.8 at 24,576 x 4,096; 256 rows 19.1 / 16.3 at 4,096 x 12,288 and
+    // 30.5 / 16.3 at 24,576 x 4,096; 512 rows 5.1 / 5.7 at 1,024 x 1,024, 11.1 / 9.2 at 4,096 x 4,096, 16.7 / 27.3 at 1,000 x 25,600.
     const bool whole = EPI == 2 || (((uintptr_t)p.out | (size_t)p.ldc * (EPI == 0 ? 2 : 4)) & 15) == 0;
     double clocks = few - 3500;
     for (int bn : {192, 256, 384}) {
