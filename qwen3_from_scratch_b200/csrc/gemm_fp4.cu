@@ -275,7 +275,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     if (split > 1) mbar_expect_tx(sums_full, (uint32_t)(split * (((rows_here - rank + split - 1) * shape.split_inverse) >> 16) * bn * 4));
   }
   __syncthreads();
-  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for before anything is sent
+  if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // waited for before anything is sent
 
   if (warp == 0) {
     // Where w is known not to come from the kernel before, its part of the ring's first round goes out ahead of the wait.
@@ -365,11 +365,17 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   } else {
     pdl_wait();
   }
+  // A gate's rows are finished either by sixteen lanes to 64 columns (below, 0.7 us for each dozen rows of 64 columns) or, where they
+  // are more than a few, by a lane to a row straight from the accumulator (24,576 x 4,096, us: 8 rows 13.7 and 15.7, 24 rows 15.6 both,
+  // 64 rows 21.4 and 16.2, 128 rows 30.6 and 18.5).
+  const bool by_rows = EPI == 2 && split == 1 && rows_here > 24;
   // Every thread gets here, whatever was given up, so the cluster's barrier needs no bound.
   if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   float* const sums = split > 1 ? received : reinterpret_cast<float*>(smem_raw);  // alone: over the ring, which nothing reads by then
-  if (warp >= 2 && aligned) {
+  if ((warp >= 2 || by_rows) && aligned) {
     const int quarter = warp & 3, row = quarter * 32 + lane;
+    // by rows, the first two warps, whose own work is done, take every second 64 columns of rows 0 .. 63
+    const int first_col = warp < 2 ? 64 : 0, next_col = by_rows && quarter < 2 ? 128 : 64;
     if (!warp_wait(acc_full, 0, &abort_flag)) {
       if (lane == 0) {
         abort_flag = 1;
@@ -383,12 +389,14 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       const uint32_t to = split > 1 ? cluster_addr(s_addr(received + (rank * shape.slots + slot) * bn), owner) : 0;
       const uint32_t bar = split > 1 ? cluster_addr(s_addr(sums_full), owner) : 0;
 #pragma unroll 1
-      for (int c0 = 0; c0 < bn; c0 += 64) {
+      for (int c0 = first_col; c0 < bn; c0 += next_col) {
         uint32_t v[2][32];
         tmem_ld_32(acc + (uint32_t)c0, v[0]);
         tmem_ld_32(acc + (uint32_t)c0 + 32, v[1]);
         tmem_wait_ld();
-        if (row < rows_here) {
+        if (EPI == 2 && by_rows) {
+          if (row < rows_here && n0 + c0 < p.N) f4_gated_block(v[0], v[1], p, m0 + row, n0 + c0);
+        } else if (row < rows_here) {
           if (split > 1) {
 #pragma unroll
             for (int j = 0; j < 16; ++j)
@@ -422,7 +430,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   // Sixteen lanes finish 64 columns of a row, four to a lane.  The blocks' sums are added in the order of their ranges of k.
   const int inner = p.N / 2, out_across = fp4_tiles(inner), blocks = (inner + FP4_BLOCK - 1) / FP4_BLOCK;
   const int groups = bn / 64, my_rows = ((rows_here - rank + split - 1) * shape.split_inverse) >> 16;
-  const int items = my_rows * groups, l = lane & 15;
+  const int items = by_rows ? 0 : my_rows * groups, l = lane & 15;
   for (int i0 = warp * 2; i0 < items; i0 += 2 * (F4_FEW_THREADS / 32)) {
     const int item = min(i0 + (lane >> 4), items - 1);  // lanes without an item of their own do the last one again
     const int slot = groups == 1 ? item : groups == 2 ? item >> 1 : item / 3, g = item - slot * groups;
@@ -802,14 +810,19 @@ static int f4_scale_map(CUtensorMap* map, const void* ptr, uint64_t tiles, uint6
   return r == CUDA_SUCCESS ? 0 : Q3_ERR_DRIVER;
 }
 
+template <typename Kernel>
+static cudaError_t f4_few_configure(Kernel kernel) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024);
+  // a kernel that asks for less keeps its SM from taking a block of one that asks for more beside its own
+  return e != cudaSuccess ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+}
+
 template <int EPI>
 static int gemm_fp4_few_launch(const CUtensorMap& map_x, const CUtensorMap& map_w, const F4Args& p, const F4FewShape& shape, int early,
                                int* status, cudaStream_t stream) {
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(gemm_fp4_few_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024);
-    if (e == cudaSuccess)  // a kernel that asks for less keeps its SM from taking a block of one that asks for more beside its own
-      e = cudaFuncSetAttribute(gemm_fp4_few_kernel<EPI>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    const cudaError_t e = f4_few_configure(gemm_fp4_few_kernel<EPI>);
     if (e != cudaSuccess) return (int)e;
     configured = true;
   }
@@ -821,18 +834,47 @@ static int gemm_fp4_few_launch(const CUtensorMap& map_x, const CUtensorMap& map_
   return code ? code : last;
 }
 
+// How many clusters of 1 to 8 blocks, one to an SM, the device runs at a time: 148, 74, 45, 33, 26, 22, 15 and 15 on 148 SMs, as a
+// cluster's SMs are of one group.  (1 x 5,120 x 25,600 with its 27 tiles of 192 rows shared out among 5 blocks each: 21.5 us, the
+// last cluster alone in a second round; as 40 tiles of 128 among 3: 14.5.)
+static const int* f4_few_slots() {
+  static int slots[64][F4_FEW_MAX_SPLIT + 1] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  for (int split = F4_FEW_MAX_SPLIT; slots[dev][1] == 0; --split) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(split * sm_count());
+    cfg.blockDim = dim3(F4_FEW_THREADS);
+    cfg.dynamicSmemBytes = 160 * 1024;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = split;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (f4_few_configure(gemm_fp4_few_kernel<0>) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, gemm_fp4_few_kernel<0>, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = sm_count() / split;
+    }
+    slots[dev][split] = n > 0 ? n : 1;
+  }
+  return slots[dev];
+}
+
 // The few-tokens kernel's tiles.  Blocks run one to an SM in rounds; a round takes its stages times what issuing one takes (clocks,
 // measured on one SM: 386, 415 and 470 for 64, 128 and 192 rows of w), and sharing out k costs the sending and adding of sums.
 static F4FewShape f4_few_shape(int T, int N, int K, double* clocks) {
   F4FewShape best{};
   double best_cost = 0, best_rounds = 0;
-  const int sms = sm_count(), k_stages = (fp4_tiles(K) + 1) / 2, rows = T < F4_BM ? T : F4_BM;
+  const int k_stages = (fp4_tiles(K) + 1) / 2, rows = T < F4_BM ? T : F4_BM, *const slots = f4_few_slots();
   for (int bn = 64; bn <= 192; bn += 64) {
     const long long tiles = (long long)((N + bn - 1) / bn) * ((T + F4_BM - 1) / F4_BM);
     for (int split = 1; split <= F4_FEW_MAX_SPLIT && split <= k_stages; ++split) {
       const int depth = (k_stages + split - 1) / split;
       if ((split - 1) * depth >= k_stages) continue;  // no block without a stage
-      const double rounds = (double)((tiles * split + sms - 1) / sms);
+      const double rounds = (double)((tiles + slots[split] - 1) / slots[split]);
       const double cost = rounds * (depth * (bn == 64 ? 386 : bn == 128 ? 415 : 470) + (split > 1 ? 600 + rows * bn / 2 : 0));
       if (best.bn == 0 || cost < best_cost) {
         best_cost = cost;
@@ -859,8 +901,8 @@ static F4FewShape f4_few_shape(int T, int N, int K, double* clocks) {
     if (room > 160 * 1024 || ((best.stages >= 3 || best.stages == best.depth) && best.ring_bytes() >= alone)) break;
   }
   while (best.ring_bytes() < alone) ++best.stages;
-  // What it takes, for the choice between the kernels: with many rows a stage takes as long as its bytes do, some 30 a clock.
-  const int issue = best.bn == 64 ? 386 : best.bn == 128 ? 415 : 470, bytes = best.stage_bytes() / 30;
+  // What it takes, for the choice between the kernels: with many rows a stage takes as long as its bytes do, some 34 a clock.
+  const int issue = best.bn == 64 ? 386 : best.bn == 128 ? 415 : 470, bytes = best.stage_bytes() / 34;
   *clocks = best_cost + best_rounds * best.depth * (bytes > issue ? bytes - issue : 0);
   return best;
 }
@@ -931,10 +973,11 @@ template <int EPI>
 static int gemm_fp4(const void* x_codes, const void* w_codes, const F4Args& p, int form, int early, int* status, cudaStream_t stream) {
   double few = 0;
   const F4FewShape shape = f4_few_shape(p.T, p.N, p.K, &few);
-  if (form == 0 && p.T >= F4_BM) {
+  if (form == 0 && p.T > 64) {
     // Pairs of CTAs where their rounds, and some 3,500 clocks that their start and end take longer, are fewer clocks.  Measured, few
-    // / pairs, us: 128 rows 9.0 / 8.4 at 4,096 x 4,096, 18.3 / 16.8 at 24,576 x 4,096; 256 rows 19.1 / 16.3 at 4,096 x 12,288 and
-    // 30.5 / 16.3 at 24,576 x 4,096; 512 rows 5.1 / 5.7 at 1,024 x 1,024, 11.1 / 9.2 at 4,096 x 4,096, 16.7 / 27.3 at 1,000 x 25,600.
+    // / pairs, us: 72 rows 14.9 / 15.2 at 24,576 x 4,096, 28.7 / 30.2 at 51,200 x 5,120; 96 rows 35.1 / 31.3 there, 8.7 / 8.1 at
+    // 4,096 x 4,096, 11.8 / 15.4 at 4,096 x 12,288; 128 rows 22.7 / 28.7 at 5,120 x 25,600; 200 rows 27.2 / 16.1 at 24,576 x 4,096,
+    // 18.7 / 16.0 at 4,096 x 12,288; 512 rows 5.1 / 5.7 at 1,024 x 1,024, 11.1 / 9.2 at 4,096 x 4,096.
     const bool whole = EPI == 2 || (((uintptr_t)p.out | (size_t)p.ldc * (EPI == 0 ? 2 : 4)) & 15) == 0;
     double clocks = few - 3500;
     for (int bn : {192, 256, 384}) {

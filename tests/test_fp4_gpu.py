@@ -286,6 +286,37 @@ def test_gated_product(act, rows, inner, width):
         assert pad_is_zero(r), form
 
 
+@pytest.mark.parametrize("rows", [24, 25, 32, 33, 63, 64, 65, 96, 127, 128, 129, 152, 200])
+@pytest.mark.parametrize("inner,width", [(8, 40), (24, 256), (72, 200), (104, 256), (136, 64), (4104, 1024)])
+def test_gated_product_of_a_few_tiles_of_rows(rows, inner, width):
+    """Rows that are finished by sixteen lanes and rows that a lane finishes alone, on both sides of every count where the one takes
+    over from the other or the next warp's rows begin, with last blocks that are not full."""
+    x, xv = held(normal(rows, width, rows))
+    w, wv = held(interleaved(normal(inner, width, 1, False), normal(inner, width, 2, False)) * width ** -0.5)
+    a, slack = gated_bounds(xv, wv, "silu")
+    low, high = plain.between(a, slack)
+    r, st = junk_rows(rows, inner), status()
+    ops().fp4_gated_product(x, w, r, st, form="few")
+    got, _ = plain.read(r.codes, r.scales, inner)
+    assert int(st.item()) == 0
+    assert bool(((got >= low) & (got <= high)).all())
+    assert pad_is_zero(r)
+
+
+@pytest.mark.parametrize("rows", [20, 60, 130])
+def test_gated_product_of_a_few_tiles_of_what_is_not_finite(rows):
+    w, _ = held(normal(64, 64, 3, False))
+    values = normal(rows, 64, rows)
+    values[1, 5] = math.nan
+    x, _ = held(values)
+    r, st = junk_rows(rows, 32), status()
+    ops().fp4_gated_product(x, w, r, st, form="few")
+    assert int(st.item()) == 0
+    got, byte = plain.read(r.codes, r.scales, 32)
+    assert bool(torch.isnan(got[1]).all())
+    assert bool(torch.isfinite(got[torch.arange(rows, device=got.device) != 1]).all())
+
+
 @pytest.mark.parametrize("form", [None, "pair192", "pair256"])
 @pytest.mark.parametrize("rows", [2, 260])
 def test_gated_product_of_what_is_not_finite(rows, form):
