@@ -8,7 +8,7 @@
 //                    128-byte swizzle, and their scales in whole 512-byte tiles;
 //   warp 1           copies each tile of scales into tensor memory (tcgen05.cp, in order with the instructions of the same
 //                    thread before and behind it) and issues instructions of k = 64, four for a stage's columns;
-//   the other warps  the epilogue.
+//   the other warps  the epilogue (of the few-tokens kernel all, when the two are done).
 // An instruction reads a row's scales of k = 64 from two of the four bytes of a tensor-memory column; which two is in its
 // descriptor.  Every wait on an mbarrier is bounded, as in gemm_tc.cu.
 //
@@ -186,7 +186,9 @@ __device__ __forceinline__ void f4_gated_block(const uint32_t (&v0)[32], const u
 // The blocks of a cluster send each row of sums, by asynchronous stores that the receiver's mbarrier counts, to the block that
 // finishes that row (rank r % split).  No block reads another's memory, so none has to stay for the others: a barrier of the
 // whole cluster behind the reading took 1.1 us.  The stores take some two clocks per 16 bytes, so many rows are not shared out.
-constexpr int F4_FEW_THREADS = 192;
+// Twelve warps, four for each 64 columns of a tile: with six in all 8 x 24,576 x 4,096 took 12.35 us instead of 12.1, with a gate and
+// 64 rows 16.2 instead of 14.3.
+constexpr int F4_FEW_THREADS = 384;
 constexpr int F4_BAR_BYTES = 512;  // barriers and the address of the tensor memory, in both kernels
 constexpr int F4_FEW_MAX_STAGES = 24;
 constexpr int F4_FEW_MAX_SPLIT = 8;
@@ -365,17 +367,17 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   } else {
     pdl_wait();
   }
-  // A gate's rows are finished either by sixteen lanes to 64 columns (below, 0.7 us for each dozen rows of 64 columns) or, where they
-  // are more than a few, by a lane to a row straight from the accumulator (24,576 x 4,096, us: 8 rows 13.7 and 15.7, 24 rows 15.6 both,
-  // 64 rows 21.4 and 16.2, 128 rows 30.6 and 18.5).
-  const bool by_rows = EPI == 2 && split == 1 && rows_here > 24;
+  // A gate's rows are finished either by sixteen lanes to 64 columns (below) or, where they are more than a few, by a lane to a row
+  // straight from the accumulator (24,576 x 4,096, us: 8 rows 13.1 and 13.9, 16 rows 13.7 and 13.9, 24 rows 14.1 and 13.7, 64 rows
+  // 17.5 and 14.3, 128 rows 23.3 and 15.6).
+  const bool by_rows = EPI == 2 && split == 1 && rows_here > 16;
   // Every thread gets here, whatever was given up, so the cluster's barrier needs no bound.
   if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   float* const sums = split > 1 ? received : reinterpret_cast<float*>(smem_raw);  // alone: over the ring, which nothing reads by then
-  if ((warp >= 2 || by_rows) && aligned) {
+  // Four warps for each 64 columns of the accumulator, the first of them the last ones: by then they are done with their own work.
+  const int c0 = (F4_FEW_THREADS / 128 - 1 - (warp >> 2)) * 64;
+  if (c0 < bn && aligned) {
     const int quarter = warp & 3, row = quarter * 32 + lane;
-    // by rows, the first two warps, whose own work is done, take every second 64 columns of rows 0 .. 63
-    const int first_col = warp < 2 ? 64 : 0, next_col = by_rows && quarter < 2 ? 128 : 64;
     if (!warp_wait(acc_full, 0, &abort_flag)) {
       if (lane == 0) {
         abort_flag = 1;
@@ -384,33 +386,29 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       __syncwarp();
     } else if (quarter * 32 < rows_here) {
       tcgen05_fence_after();
-      const uint32_t acc = *(volatile uint32_t*)tmem_holder + ((uint32_t)(quarter * 32) << 16);
-      const int slot = (row * shape.split_inverse) >> 16, owner = row - slot * split;  // row / split, row % split
-      const uint32_t to = split > 1 ? cluster_addr(s_addr(received + (rank * shape.slots + slot) * bn), owner) : 0;
-      const uint32_t bar = split > 1 ? cluster_addr(s_addr(sums_full), owner) : 0;
-#pragma unroll 1
-      for (int c0 = first_col; c0 < bn; c0 += next_col) {
-        uint32_t v[2][32];
-        tmem_ld_32(acc + (uint32_t)c0, v[0]);
-        tmem_ld_32(acc + (uint32_t)c0 + 32, v[1]);
-        tmem_wait_ld();
-        if (EPI == 2 && by_rows) {
-          if (row < rows_here && n0 + c0 < p.N) f4_gated_block(v[0], v[1], p, m0 + row, n0 + c0);
-        } else if (row < rows_here) {
-          if (split > 1) {
+      const uint32_t acc = *(volatile uint32_t*)tmem_holder + ((uint32_t)(quarter * 32) << 16) + c0;
+      uint32_t v[2][32];
+      tmem_ld_32(acc, v[0]);
+      tmem_ld_32(acc + 32, v[1]);
+      tmem_wait_ld();
+      if (row >= rows_here) {
+      } else if (EPI == 2 && by_rows) {
+        if (n0 + c0 < p.N) f4_gated_block(v[0], v[1], p, m0 + row, n0 + c0);
+      } else if (split > 1) {
+        const int slot = (row * shape.split_inverse) >> 16, owner = row - slot * split;  // row / split, row % split
+        const uint32_t to = cluster_addr(s_addr(received + (rank * shape.slots + slot) * bn), owner);
+        const uint32_t bar = cluster_addr(s_addr(sums_full), owner);
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              st_async_v4(to + (c0 + 4 * j) * 4, v[j / 8][4 * (j % 8)], v[j / 8][4 * (j % 8) + 1], v[j / 8][4 * (j % 8) + 2],
-                          v[j / 8][4 * (j % 8) + 3], bar);
-          } else {  // rows bn + 4 values apart, off each other's banks
+        for (int j = 0; j < 16; ++j)
+          st_async_v4(to + (c0 + 4 * j) * 4, v[j / 8][4 * (j % 8)], v[j / 8][4 * (j % 8) + 1], v[j / 8][4 * (j % 8) + 2],
+                      v[j / 8][4 * (j % 8) + 3], bar);
+      } else {  // rows bn + 4 values apart, off each other's banks
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              *reinterpret_cast<uint4*>(sums + row * (bn + 4) + c0 + 4 * j) =
-                  make_uint4(v[j / 8][4 * (j % 8)], v[j / 8][4 * (j % 8) + 1], v[j / 8][4 * (j % 8) + 2], v[j / 8][4 * (j % 8) + 3]);
-          }
-        }
-        __syncwarp();
+        for (int j = 0; j < 16; ++j)
+          *reinterpret_cast<uint4*>(sums + row * (bn + 4) + c0 + 4 * j) =
+              make_uint4(v[j / 8][4 * (j % 8)], v[j / 8][4 * (j % 8) + 1], v[j / 8][4 * (j % 8) + 2], v[j / 8][4 * (j % 8) + 3]);
       }
+      __syncwarp();
     }
   }
   tcgen05_fence_before();
@@ -901,8 +899,8 @@ static F4FewShape f4_few_shape(int T, int N, int K, double* clocks) {
     if (room > 160 * 1024 || ((best.stages >= 3 || best.stages == best.depth) && best.ring_bytes() >= alone)) break;
   }
   while (best.ring_bytes() < alone) ++best.stages;
-  // What it takes, for the choice between the kernels: with many rows a stage takes as long as its bytes do, some 34 a clock.
-  const int issue = best.bn == 64 ? 386 : best.bn == 128 ? 415 : 470, bytes = best.stage_bytes() / 34;
+  // What it takes, for the choice between the kernels: with many rows a stage takes as long as its bytes do, some 40 a clock.
+  const int issue = best.bn == 64 ? 386 : best.bn == 128 ? 415 : 470, bytes = best.stage_bytes() / 40;
   *clocks = best_cost + best_rounds * best.depth * (bytes > issue ? bytes - issue : 0);
   return best;
 }
@@ -974,12 +972,13 @@ static int gemm_fp4(const void* x_codes, const void* w_codes, const F4Args& p, i
   double few = 0;
   const F4FewShape shape = f4_few_shape(p.T, p.N, p.K, &few);
   if (form == 0 && p.T > 64) {
-    // Pairs of CTAs where their rounds, and some 3,500 clocks that their start and end take longer, are fewer clocks.  Measured, few
-    // / pairs, us: 72 rows 14.9 / 15.2 at 24,576 x 4,096, 28.7 / 30.2 at 51,200 x 5,120; 96 rows 35.1 / 31.3 there, 8.7 / 8.1 at
-    // 4,096 x 4,096, 11.8 / 15.4 at 4,096 x 12,288; 128 rows 22.7 / 28.7 at 5,120 x 25,600; 200 rows 27.2 / 16.1 at 24,576 x 4,096,
-    // 18.7 / 16.0 at 4,096 x 12,288; 512 rows 5.1 / 5.7 at 1,024 x 1,024, 11.1 / 9.2 at 4,096 x 4,096.
+    // Pairs of CTAs where their rounds, and some 3,500 clocks that their start and end take longer (5,500 with a gate), are fewer
+    // clocks.  Measured, few / pairs, us: 72 rows 28.0 / 30.2 at 51,200 x 5,120; 96 rows 14.6 / 15.5 at 24,576 x 4,096, 32.4 / 31.2
+    // at 51,200 x 5,120, 11.4 / 15.4 at 4,096 x 12,288; 128 rows 22.3 / 28.8 at 5,120 x 25,600; 200 rows 24.5 / 16.7 at 24,576 x
+    // 4,096, 18.6 / 16.1 at 4,096 x 12,288; 400 rows 4.9 / 5.7 at 1,024 x 1,024, 9.8 / 9.1 at 4,096 x 4,096, 20.9 / 17.6 at 4,096 x
+    // 12,288; with a gate 128 rows 15.3 / 17.0 at 24,576 x 4,096, 400 rows 9.8 / 10.6 at 4,096 x 4,096 and 42.7 / 25.1 at 24,576 x 4,096.
     const bool whole = EPI == 2 || (((uintptr_t)p.out | (size_t)p.ldc * (EPI == 0 ? 2 : 4)) & 15) == 0;
-    double clocks = few - 3500;
+    double clocks = few - (EPI == 2 ? 5500 : 3500);
     for (int bn : {192, 256, 384}) {
       if (bn == 384 && EPI != 0) break;
       const double c = f4_pair_cost(p.T, p.N, p.K, bn, EPI, whole);
