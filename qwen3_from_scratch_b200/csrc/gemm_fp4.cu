@@ -100,48 +100,149 @@ __device__ __forceinline__ void f4_pack(const uint32_t (&v0)[32], const uint32_t
     w[16 + i] = pack2(v1[2 * i], v1[2 * i + 1]);
   }
 }
-// 128 bytes of results (32 float32 or 64 bfloat16 columns from `col` on) of each of the warp's 32 rows, a row to a lane, by way of
-// 4 KB of shared memory: there the lanes change places, so that eight of them store the 128 bytes of a row side by side.  Storing
-// from the accumulator's own order, 16 bytes of 32 different rows at a time, took as long as the main loop (2,048 x 24,576 x
-// 4,096: 90 us with it, 64 without any stores).  16-byte piece c of row r lies at r * 128 + ((c ^ (r % 8)) * 16), off the banks of
-// its neighbours both ways.
+// Where a warp of the epilogue puts the results of its 32 rows, 128 bytes of each (32 float32 or 64 bfloat16 columns) at a time, a
+// row to a lane, by way of 4 KB of shared memory: there the lanes change places, so that eight of them store the 128 bytes of a row
+// side by side.  Storing from the accumulator's own order, 16 bytes of 32 different rows at a time, took as long as the main loop
+// (2,048 x 24,576 x 4,096: 90 us with it, 64 without any stores).  16-byte piece c of row r lies at r * 128 + ((c ^ (r % 8)) * 16),
+// off the banks of its neighbours both ways.
+//
+// Memory takes whole sectors of 32 bytes far better than parts of them (8,000 x 16,001 x 64, float32: 101 us with 16,000 columns,
+// 258 with a piece's first and last values stored one by one).  So where rows are off a sector's boundary, what leaves is the 128
+// bytes up to the last boundary: each lane holds back the last bytes of its row and puts them in front of the next ones.
 template <int EPI>
-__device__ __forceinline__ void f4_store_rows(const uint32_t (&w)[32], unsigned char* stage, const F4Args& p, int row0, int col, int lane) {
+struct F4RowStore {
   using OutT = typename std::conditional<EPI == 0, __nv_bfloat16, float>::type;
-  constexpr int PER = 16 / sizeof(OutT);  // values of a piece
+  unsigned char* stage;
+  unsigned char* first;  // the warp's first row, first column
+  size_t pitch;          // bytes from a row to the next
+  int rows, bytes;       // rows, and bytes of each, that are results
+  int at;                // bytes of each row that have come
+  bool whole;            // no row is off a sector's boundary, all columns are results (uniform over the warp)
+  uint32_t held[8];      // the last 32 bytes that came
+
+  __device__ __forceinline__ F4RowStore(const F4Args& p, unsigned char* stage_, int row0, int col, int cols)
+      : stage(stage_), first((unsigned char*)p.out + ((size_t)row0 * p.ldc + col) * sizeof(OutT)), pitch((size_t)p.ldc * sizeof(OutT)),
+        rows(min(32, p.T - row0)), bytes(min(cols, p.N - col) * (int)sizeof(OutT)), at(0),
+        whole(col + cols <= p.N && (((uintptr_t)p.out | (size_t)p.ldc * sizeof(OutT)) & 31) == 0) {}
+
+  // The next 128 bytes of each row.
+  __device__ __forceinline__ void push(const uint32_t (&w)[32], int lane) {
+    if (at >= bytes) return;  // uniform over the warp
+    if (whole) {
+      put(w, lane, 8);
+      const int c = lane & 7;
+      unsigned char* to = first + (lane >> 3) * pitch + at + c * 16;
 #pragma unroll
-  for (int c = 0; c < 8; ++c)
-    *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-  __syncwarp();
-  OutT* dst = (OutT*)p.out + (size_t)row0 * p.ldc + col;
-  const int rows = min(32, p.T - row0);
-  if (col + 8 * PER <= p.N && (((uintptr_t)p.out | (size_t)p.ldc * sizeof(OutT)) & 15) == 0) {  // uniform over the warp
-    const int c = lane & 7;
-    dst += (size_t)(lane >> 3) * p.ldc + c * PER;
+      for (int i = 0; i < 8; ++i, to += 4 * pitch) {
+        const int r = 4 * i + (lane >> 3);
+        if (r < rows) *reinterpret_cast<uint4*>(to) = piece(r, c);
+      }
+    } else {
+      uint32_t x[40];
 #pragma unroll
-    for (int i = 0; i < 8; ++i, dst += 4 * p.ldc) {
-      const int r = 4 * i + (lane >> 3);
-      if (r < rows) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
+      for (int j = 0; j < 40; ++j) x[j] = j < 8 ? held[j] : w[j - 8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) held[j] = w[24 + j];
+      shift(x, lane);
+      uint32_t y[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) y[j] = x[8 + j];
+      put(y, lane, 8);
+      leave(lane, true);
     }
-  } else {  // rows off a 16-byte boundary, or the last columns: a word of each row to a lane
-#pragma unroll 4
-    for (int r = 0; r < rows; ++r, dst += p.ldc) {
-      const uint32_t x = *reinterpret_cast<const uint32_t*>(stage + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-      if (EPI == 1) {
-        if (col + lane < p.N) reinterpret_cast<uint32_t*>(dst)[lane] = x;
-      } else {
-        uint16_t* const two = reinterpret_cast<uint16_t*>(dst) + 2 * lane;
-        if (((uintptr_t)two & 3) == 0 && col + 2 * lane + 1 < p.N) {
-          *reinterpret_cast<uint32_t*>(two) = x;
-        } else {
-          if (col + 2 * lane < p.N) two[0] = (uint16_t)x;
-          if (col + 2 * lane + 1 < p.N) two[1] = (uint16_t)(x >> 16);
+    __syncwarp();
+    at += 128;
+  }
+  // What is still held back.
+  __device__ __forceinline__ void end(int lane) {
+    if (whole || at == 0) return;  // uniform over the warp
+    uint32_t x[16], y[32];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = j < 8 ? held[j] : 0u;
+    shift(x, lane);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) y[j] = j < 8 ? x[8 + j] : 0u;
+    put(y, lane, 2);
+    leave(lane, false);
+    __syncwarp();
+  }
+
+ private:
+  __device__ __forceinline__ uint4 piece(int r, int c) const { return *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4)); }
+  __device__ __forceinline__ void put(const uint32_t (&y)[32], int lane, int pieces) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < pieces)
+        *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
+    __syncwarp();
+  }
+  // x, from its ninth word on, moves up by as many bytes as the lane's row is behind a sector's boundary.
+  template <int N>
+  __device__ __forceinline__ void shift(uint32_t (&x)[N], int lane) const {
+    const uint32_t m = (uint32_t)(uintptr_t)(first + lane * pitch) & 31u;
+#pragma unroll
+    for (int j = N - 1; j >= 1; --j) x[j] = m & 4 ? x[j - 1] : x[j];
+#pragma unroll
+    for (int j = N - 1; j >= 3; --j) x[j] = m & 8 ? x[j - 2] : x[j];
+#pragma unroll
+    for (int j = N - 1; j >= 7; --j) x[j] = m & 16 ? x[j - 4] : x[j];
+    if (EPI == 0) {
+#pragma unroll
+      for (int j = N - 1; j >= 8; --j) x[j] = m & 2 ? __funnelshift_r(x[j - 1], x[j], 16) : x[j];
+    }
+  }
+  // Of the 128 bytes behind the boundary (`all`; else of the first sector): what is whole by sixteen bytes to a lane, of the row's
+  // first and last sector what is the row's, a word to a lane.  Four rows' reads go out together: one by one they took longer than
+  // the stores.
+  __device__ __forceinline__ void leave(int lane, bool all) const {
+    const int c = lane & 7, len = all ? 128 : 32;
+    if (all) {
+      unsigned char* row = first + (lane >> 3) * pitch;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4 q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = piece(16 * h + 4 * i + (lane >> 3), c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i, row += 4 * pitch) {
+          const int m = (int)((uintptr_t)row & 31), lo = m - at, hi = bytes + m - at;
+          const bool ok = 16 * h + 4 * i + (lane >> 3) < rows && 32 * (c >> 1) >= lo && 32 * (c >> 1) + 32 <= hi;
+          if (ok) *reinterpret_cast<uint4*>(row - m + at + c * 16) = q[i];
+        }
+      }
+    }
+    if (at == 0) part(lane, len, true);
+    if (at + len > bytes) part(lane, len, false);
+  }
+  // The row's first sector (`low`), if a part of it is another's, or its last one, if it is another one and ends among these bytes.
+  __device__ __forceinline__ void part(int lane, int len, bool low) const {
+    const int c = lane & 7;
+    unsigned char* row = first + (lane >> 3) * pitch;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t x[4];
+      int from[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * h + 4 * i + (lane >> 3), m = (int)((uintptr_t)(row + i * 4 * pitch) & 31), hi = bytes + m - at;
+        const bool ok = r < rows && (low ? m > 0 : hi > 0 && hi < len && (hi & 31) != 0 && (at > 0 || m == 0 || hi > 32));
+        from[i] = ok ? (low ? 0 : hi & ~31) + c * 4 : -1;
+        const int word = max(from[i], 0);
+        x[i] = *reinterpret_cast<const uint32_t*>(stage + r * 128 + (((word >> 4) ^ (r & 7)) << 4) + (word & 15));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i, row += 4 * pitch) {
+        const int m = (int)((uintptr_t)row & 31), lo = m - at, hi = bytes + m - at, w = from[i];
+        unsigned char* const to = row - m + at + w;
+        if (w >= 0 && lo <= w && hi >= w + 4) *reinterpret_cast<uint32_t*>(to) = x[i];
+        if (EPI == 0) {
+          if (w >= 0 && lo <= w && hi == w + 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)x[i];
+          if (w >= 0 && lo == w + 2 && hi >= w + 4) *reinterpret_cast<uint16_t*>(to + 2) = (uint16_t)(x[i] >> 16);
         }
       }
     }
   }
-  __syncwarp();
-}
+};
 // 64 columns, gate and up in blocks of eight: a block of 32 results, their codes and scale.
 __device__ __forceinline__ void f4_gated_block(const uint32_t (&v0)[32], const uint32_t (&v1)[32], const F4Args& p, int row, int col) {
   const int inner = p.N / 2, blocks = (inner + FP4_BLOCK - 1) / FP4_BLOCK, out_across = fp4_tiles(inner), j = col / 64;
@@ -716,20 +817,8 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         if (lane == 0) f4_arrive_relaxed(cluster_addr(s_addr(&acc_empty[buf]), 0));
         __syncwarp();
       };
-      // 64 columns: what leaves
-      auto finish = [&](const uint32_t(&v0)[32], const uint32_t(&v1)[32], int col) {
-        if (row0 >= p.T || col >= p.N) return;  // uniform over the warp
-        if (EPI == 2) {
-          if (row0 + lane < p.T) f4_gated_block(v0, v1, p, row0 + lane, col);
-        } else if (EPI == 0) {
-          uint32_t w[32];
-          f4_pack(v0, v1, w);
-          f4_store_rows<EPI>(w, store, p, row0, col, lane);
-        } else {
-          f4_store_rows<EPI>(v0, store, p, row0, col, lane);
-          if (col + 32 < p.N) f4_store_rows<EPI>(v1, store, p, row0, col + 32, lane);
-        }
-      };
+      F4RowStore<EPI> to(p, store, row0, n0, 64 * pieces);
+      const bool any = row0 < p.T && n0 < p.N;  // uniform over the warp, as all that follows
       if (BN != 384) {
         uint32_t v[4][32];
 #pragma unroll
@@ -737,9 +826,28 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
           if (c < 2 * pieces) tmem_ld_32(acc + 32 * c, v[c]);
         tmem_wait_ld();
         release();
+        uint32_t w[2][32];
+        if (EPI == 0 && BN == 256) {  // here and not later, or the registers do not suffice for what follows
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            f4_pack(v[2 * c], v[2 * c + 1], w[c]);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) asm volatile("" : "+r"(w[c][j]));
+          }
+        }
 #pragma unroll
         for (int c = 0; c < 2; ++c)
-          if (c < pieces) finish(v[2 * c], v[2 * c + 1], n0 + 64 * c);
+          if (any && c < pieces) {  // 64 columns: what leaves
+            if (EPI == 2) {
+              if (row0 + lane < p.T && n0 + 64 * c < p.N) f4_gated_block(v[2 * c], v[2 * c + 1], p, row0 + lane, n0 + 64 * c);
+            } else if (EPI == 0) {
+              if (BN != 256) f4_pack(v[2 * c], v[2 * c + 1], w[c]);
+              to.push(w[c], lane);
+            } else {
+              to.push(v[2 * c], lane);
+              to.push(v[2 * c + 1], lane);
+            }
+          }
       } else {  // bfloat16 results only: a tile of 384 columns fits in the registers as such
         uint32_t v[2][2][32], w[3][32];
         tmem_ld_32(acc, v[0][0]);
@@ -757,8 +865,9 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         }
 #pragma unroll
         for (int c = 0; c < 3; ++c)
-          if (row0 < p.T && n0 + 64 * c < p.N) f4_store_rows<EPI>(w[c], store, p, row0, n0 + 64 * c, lane);
+          if (any) to.push(w[c], lane);
       }
+      if (EPI != 2 && any) to.end(lane);
     }
   }
   tcgen05_fence_before();
@@ -899,9 +1008,12 @@ static F4FewShape f4_few_shape(int T, int N, int K, double* clocks) {
     if (room > 160 * 1024 || ((best.stages >= 3 || best.stages == best.depth) && best.ring_bytes() >= alone)) break;
   }
   while (best.ring_bytes() < alone) ++best.stages;
+  // Rounds of blocks that take more than half of an SM's shared memory do not overlap (128 rows of 192 columns: some 8,000 clocks from
+  // one's start to its first stage and from its last one to its end).
+  const double apart = best.smem_bytes() > 113 * 1024 ? (best_rounds - 1) * (3000 + rows * best.bn / 5) : 0;
   // What it takes, for the choice between the kernels: with many rows a stage takes as long as its bytes do, some 40 a clock.
   const int issue = best.bn == 64 ? 386 : best.bn == 128 ? 415 : 470, bytes = best.stage_bytes() / 40;
-  *clocks = best_cost + best_rounds * best.depth * (bytes > issue ? bytes - issue : 0);
+  *clocks = best_cost + best_rounds * best.depth * (bytes > issue ? bytes - issue : 0) + apart;
   return best;
 }
 
@@ -929,14 +1041,18 @@ static int f4_pair_slots() {
 
 // Clocks of the pair kernel's rounds: its stages, and what a tile takes beside them.  Measured with 192, 256 and 384 columns, us:
 // 79, 77, 73 at 2,048 x 24,576 x 4,096, 43, 40, 53 at 2,048 x 4,096 x 12,288, 350, 341, 364 at 8,192 x 5,120 x 25,600, 16.4, 20,
-// 28 at 256 x 4,096 x 12,288 (a stage 420, 560 and 715 clocks, and 1,700, 1,200 and 3,700 a tile, fit these and ten more).  Rows
-// of results off a 16-byte boundary leave a word of each row to a lane and hold a round up further (3,000 x 9,001 x 2,560: 67 us in
-// float32 and 47 in bfloat16, 44 and 35 with 9,000 columns).
+// 28 at 256 x 4,096 x 12,288 (a stage 420, 560 and 715 clocks, and 1,700, 1,200 and 3,700 a tile, fit these and ten more).  Where k is
+// short a tile takes as long as its results do to leave: 53, 50 and 49 us at 8,000 x 16,000 x 64, in float32 105 and 101; and with
+// rows off a sector's boundary (16,001 columns) 122, 105 and 98, in float32 177 and 147.
 static double f4_pair_cost(int T, int N, int K, int bn, int epi, bool whole) {
   const long long tiles = (long long)((N + bn - 1) / bn) * ((T + 255) / 256), slots = f4_pair_slots();
   const int k_stages = (fp4_tiles(K) + 1) / 2;
   const double stage = bn == 192 ? 420 : bn == 256 ? 560 : 715, hold = bn == 192 ? 1700 : bn == 256 ? 1200 : 3700;
-  return (double)((tiles + slots - 1) / slots) * (k_stages * stage + hold + (whole ? 0 : epi == 0 ? 1700 : 6500) * (bn / 192.0));
+  double leave = bn == 192 ? 4500 : 6000;  // a gate
+  if (epi == 0) leave = whole ? (bn == 192 ? 2200 : bn == 256 ? 2700 : 3900) : (bn == 192 ? 5000 : bn == 256 ? 5600 : 7700);
+  if (epi == 1) leave = whole ? (bn == 192 ? 4300 : 5400) : (bn == 192 ? 7200 : 7900);
+  const double tile = k_stages * stage + hold;
+  return (double)((tiles + slots - 1) / slots) * (tile > leave ? tile : leave);
 }
 
 template <int EPI, int BN>
@@ -977,7 +1093,7 @@ static int gemm_fp4(const void* x_codes, const void* w_codes, const F4Args& p, i
     // at 51,200 x 5,120, 11.4 / 15.4 at 4,096 x 12,288; 128 rows 22.3 / 28.8 at 5,120 x 25,600; 200 rows 24.5 / 16.7 at 24,576 x
     // 4,096, 18.6 / 16.1 at 4,096 x 12,288; 400 rows 4.9 / 5.7 at 1,024 x 1,024, 9.8 / 9.1 at 4,096 x 4,096, 20.9 / 17.6 at 4,096 x
     // 12,288; with a gate 128 rows 15.3 / 17.0 at 24,576 x 4,096, 400 rows 9.8 / 10.6 at 4,096 x 4,096 and 42.7 / 25.1 at 24,576 x 4,096.
-    const bool whole = EPI == 2 || (((uintptr_t)p.out | (size_t)p.ldc * (EPI == 0 ? 2 : 4)) & 15) == 0;
+    const bool whole = EPI == 2 || (((uintptr_t)p.out | (size_t)p.ldc * (EPI == 0 ? 2 : 4)) & 31) == 0;
     double clocks = few - (EPI == 2 ? 5500 : 3500);
     for (int bn : {192, 256, 384}) {
       if (bn == 384 && EPI != 0) break;

@@ -213,6 +213,28 @@ def test_product_into_columns(out, rows, features, start, more):
         assert bool((wide[:, :start] == 3).all()) and bool((wide[:, end:] == 3).all()), form
 
 
+@pytest.mark.parametrize("out", list(DT))
+@pytest.mark.parametrize("rows", [1, 70, 300])
+@pytest.mark.parametrize("features", [1, 15, 33, 191, 193, 257, 385, 450, 513])
+def test_product_off_every_boundary(rows, features, out):
+    """Rows that begin at every place within 32 bytes, in rows further apart than they are long: the same bits as in rows of their own,
+    and nothing of what lies around them is touched."""
+    x, _ = held(normal(rows, 96, rows))
+    w, _ = held(normal(features, 96, 2, spread=False))
+    for form in ("few", "pair192", "pair256", "pair384"):
+        if form == "pair384" and out == "float32":
+            continue
+        own = torch.empty(rows, (features + 15) // 16 * 16, dtype=DT[out], device="cuda")
+        ops().fp4_product(x, w, own[:, :features], status(), form=form)
+        for start in range(0, 17):
+            pitch = features + start + (5 * start + 3) % 17
+            wide = torch.full((rows + 2, pitch), 3.0, dtype=DT[out], device="cuda")
+            ops().fp4_product(x, w, wide[1:-1, start:start + features], status(), form=form)
+            assert torch.equal(wide[1:-1, start:start + features], own[:, :features]), (form, start)
+            wide[1:-1, start:start + features] = 3.0
+            assert bool((wide == 3).all()), (form, start)
+
+
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("rows,features", [(5, 200), (300, 700)])
 def test_product_rows_beyond_the_first(rows, features, form):
