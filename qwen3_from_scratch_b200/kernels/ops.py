@@ -3144,7 +3144,7 @@ def rotate_columns(x: torch.Tensor, column: int, heads: int, dim: int, dims: int
 # ------------------------------------------------------------------ rows held in microscaled 4-bit floating point
 FP4_BLOCK = 32             # values of a row that share a scale
 FP4_MAX_NORM_WIDTH = 32768  # widest row of fp4_add_rmsnorm
-FP4_GATES = ("silu", "relu", "gelu_tanh")
+FP4_GATES = {name: ACTIVATIONS[name] for name in ("silu", "relu", "gelu_tanh")}
 
 
 class Fp4Rows(NamedTuple):
@@ -3215,22 +3215,27 @@ def fp4_quantise(x: torch.Tensor, out: Fp4Rows, values: Optional[torch.Tensor] =
         _done("fp4_quantise", code, f"{T} rows of {K}")
 
 
+def _check_rows(name: str, t: torch.Tensor, dtype: torch.dtype, size: torch.Size) -> None:
+    if not (t.is_cuda and t.dtype is dtype and t.is_contiguous()):
+        _check(name, t, dtype)
+    if t.shape != size:
+        raise KernelError(f"{name}: {tuple(t.shape)}, the stream is {tuple(size)}")
+
+
 def _check_fp4_stream(name: str, stream: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor,
-                      stream_out: Optional[torch.Tensor], dtype: torch.dtype) -> Tuple[int, int]:
-    size = stream.shape
-    _check(f"{name}.stream", stream, torch.float32)
-    _check(f"{name}.weight", weight, torch.float32)
-    if len(size) != 2 or weight.shape[-1] != size[1] or weight.numel() != size[1]:
+                      stream_out: Optional[torch.Tensor], dtype: torch.dtype) -> torch.Size:
+    size, f32 = stream.shape, torch.float32
+    if not (stream.is_cuda and weight.is_cuda and stream.dtype is weight.dtype is f32 and stream.is_contiguous()
+            and weight.is_contiguous()):
+        _check(f"{name}.stream", stream, f32)
+        _check(f"{name}.weight", weight, f32)
+    if len(size) != 2 or weight.numel() != size[1] or weight.shape[-1] != size[1]:
         raise KernelError(f"{name}: weight {tuple(weight.shape)}, stream {tuple(size)}")
     if delta is not None:
-        _check(f"{name}.delta", delta, dtype)
-        if delta.shape != size:
-            raise KernelError(f"{name}: delta {tuple(delta.shape)} vs stream {tuple(size)}")
+        _check_rows(f"{name}.delta", delta, dtype, size)
     if stream_out is not None:
-        _check(f"{name}.stream_out", stream_out, torch.float32)
-        if stream_out.shape != size:
-            raise KernelError(f"{name}: stream_out {tuple(stream_out.shape)} vs stream {tuple(size)}")
-    return size[0], size[1]
+        _check_rows(f"{name}.stream_out", stream_out, f32, size)
+    return size
 
 
 def fp4_add_rmsnorm(stream: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, out: Fp4Rows, eps: float,
@@ -3242,7 +3247,8 @@ def fp4_add_rmsnorm(stream: torch.Tensor, delta: Optional[torch.Tensor], weight:
     code = library().q3_fp4_add_rmsnorm(stream.data_ptr(), _ptr(delta), F32 if delta is None else dtype_tag(delta.dtype),
                                         weight.data_ptr(), (stream if stream_out is None else stream_out).data_ptr(),
                                         out.codes.data_ptr(), out.scales.data_ptr(), T, H, float(eps), _stream())
-    _done("fp4_add_rmsnorm", code, f"width {H}")
+    if code:
+        _done("fp4_add_rmsnorm", code, f"width {H}")
 
 
 FP4_FORMS = {None: 0, "few": 1, "pair192": 192, "pair256": 256, "pair384": 384}
@@ -3267,9 +3273,10 @@ def fp4_product(x: Fp4Rows, w: Fp4Rows, out: torch.Tensor, status: torch.Tensor,
 
 
 def _fp4_gate(name: str, activation: str) -> int:
-    if activation not in FP4_GATES:
-        raise KernelError(f"{name}: no gate {activation!r} (there are {FP4_GATES})")
-    return activation_code(activation, gate=True)
+    code = FP4_GATES.get(activation)
+    if code is None:
+        raise KernelError(f"{name}: no gate {activation!r} (there are {tuple(FP4_GATES)})")
+    return code
 
 
 def fp4_gated_product(x: Fp4Rows, w: Fp4Rows, out: Fp4Rows, status: torch.Tensor, activation: str = "silu",
@@ -3283,7 +3290,8 @@ def fp4_gated_product(x: Fp4Rows, w: Fp4Rows, out: Fp4Rows, status: torch.Tensor
                                           out.codes.data_ptr(), out.scales.data_ptr(), x.rows, w.rows, x.width,
                                           _fp4_gate("fp4_gated_product", activation), FP4_FORMS[form], status.data_ptr(),
                                           _stream())
-    _done("fp4_gated_product", code, f"T {x.rows} N {w.rows} K {x.width}")
+    if code:
+        _done("fp4_gated_product", code, f"T {x.rows} N {w.rows} K {x.width}")
 
 
 def fp4_feed_forward(stream: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, eps: float, gate_up: Fp4Rows,
@@ -3291,18 +3299,17 @@ def fp4_feed_forward(stream: torch.Tensor, delta: Optional[torch.Tensor], weight
                      activation: str = "silu", stream_out: Optional[torch.Tensor] = None) -> None:
     """A gated feed-forward behind its norm in one call: ``fp4_add_rmsnorm`` into ``normed`` [T, H], ``fp4_gated_product``
     with ``gate_up`` [2 I, H] into ``gated`` [T, I], and out[T, H] = gated @ down[H, I]^T; delta has the dtype of out."""
-    _check("fp4_feed_forward.out", out)
-    T, H = _check_fp4_stream("fp4_feed_forward", stream, delta, weight, stream_out, out.dtype)
+    size = T, H = _check_fp4_stream("fp4_feed_forward", stream, delta, weight, stream_out, out.dtype)
+    _check_rows("fp4_feed_forward.out", out, out.dtype, size)
     inner = down.width
     _check_fp4("fp4_feed_forward.gate_up", gate_up, H, 2 * inner)
     _check_fp4("fp4_feed_forward.down", down, inner, H)
     _check_fp4("fp4_feed_forward.normed", normed, H, T)
     _check_fp4("fp4_feed_forward.gated", gated, inner, T)
-    if tuple(out.shape) != (T, H):
-        raise KernelError(f"fp4_feed_forward: out {tuple(out.shape)} vs stream {(T, H)}")
     code = library().q3_fp4_feed_forward(
         stream.data_ptr(), _ptr(delta), weight.data_ptr(), (stream if stream_out is None else stream_out).data_ptr(), float(eps),
         gate_up.codes.data_ptr(), gate_up.scales.data_ptr(), down.codes.data_ptr(), down.scales.data_ptr(),
         normed.codes.data_ptr(), normed.scales.data_ptr(), gated.codes.data_ptr(), gated.scales.data_ptr(), out.data_ptr(),
         dtype_tag(out.dtype), T, H, inner, _fp4_gate("fp4_feed_forward", activation), status.data_ptr(), _stream())
-    _done("fp4_feed_forward", code, f"T {T} H {H} I {inner}")
+    if code:
+        _done("fp4_feed_forward", code, f"T {T} H {H} I {inner}")

@@ -91,7 +91,7 @@ class GatedMLP(FeedForward):
         """Weights as ``ops.Fp4Rows``, gate and up rows alternating in blocks of eight, and room for the rounded activations."""
         h, i = self.hidden_size, self.intermediate_size
         if self.has_bias or self.activation not in ops.FP4_GATES or i % 8:
-            raise ValueError(f"feed-forward {self.name}: fp4 weights take no biases, one of {ops.FP4_GATES} as the gate and a width in "
+            raise ValueError(f"feed-forward {self.name}: fp4 weights take no biases, one of {tuple(ops.FP4_GATES)} as the gate and a width in "
                              f"multiples of 8, not {self.activation}, {i}{' and biases' if self.has_bias else ''}")
         gate, up = weights.pop(self.tensors["gate"]), weights.pop(self.tensors["up"])
         merged = torch.cat([gate.view(i // 8, 8, h), up.view(i // 8, 8, h)], dim=1).reshape(2 * i, h)
