@@ -35,6 +35,12 @@ __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t top) {
   const int b = (int)((top + 0x1fffffu) >> 23) - 2;  // one more where the significand is above 1.75, then 7 = 1.75 x 2^2
   return b < 0 ? 0u : (uint32_t)b;
 }
+// The larger of `top` and |v|, bits for bits; a NaN stays one.
+__device__ __forceinline__ uint32_t fp4_top(uint32_t top, float v) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(fabsf(v)), "f"(__uint_as_float(top)));
+  return __float_as_uint(m);
+}
 // 1 / X.  b is at most 253, so this is a normal number; 255 gives 0, which leaves zeros (and NaN) for the codes.
 __device__ __forceinline__ float fp4_inverse_scale(uint32_t b) { return b == 255u ? 0.f : __uint_as_float((254u - b) << 23); }
 
@@ -61,7 +67,7 @@ __device__ __forceinline__ uint32_t fp4_pack2(float lo, float hi) {
 __device__ __forceinline__ uint32_t fp4_round8(const float (&v)[8], uint32_t* scale_byte) {
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  for (int i = 0; i < 8; ++i) top = fp4_top(top, v[i]);
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   const uint32_t b = fp4_scale_byte(top);

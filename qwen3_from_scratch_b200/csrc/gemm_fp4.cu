@@ -77,19 +77,29 @@ __device__ __forceinline__ bool warp_wait_cluster(uint64_t* bar, uint32_t parity
   return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity, abort_flag));
 }
 
-// a[i] = act(g[i]) * u[i].  SiLU and GELU's tanh form are g sigmoid(z): (1 + tanh(y)) / 2 = sigmoid(2 y).  The fast exponential and
-// division are off by a few times 2^-23, which moves a result across a boundary between two codes once in some 10^5 values; the
-// exact ones, one value after another, took 1.2 us of a call's last 1.9 where a lane has four values to do.
+// a[i] = act(g[i]) * u[i].  SiLU and GELU's tanh form are g sigmoid(z) = g / (1 + 2^(-z log2 e)), as (1 + tanh(y)) / 2 = sigmoid(2 y).
+// The fast power and reciprocal are off by a few times 2^-23, which moves a result across a boundary between two codes once in
+// some 10^5 values; the exact ones, one value after another, took 1.2 us of a call's last 1.9 where a lane has four values to do.
+// A loop for each gate, with nothing in it that the others need: where k is short, a gate is what bounds the call.
+__device__ __forceinline__ float f4_over_one_and_power(float g, float e) {  // g / (1 + 2^e)
+  float t, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(e));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + t));
+  return g * r;
+}
 template <int N>
 __device__ __forceinline__ void f4_gate(const float (&g)[N], const float (&u)[N], int act, float (&a)[N]) {
-  if (act == Q3_ACT_RELU) {
+  constexpr float LOG2E = 1.4426950408889634f, Z = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+  if (act == Q3_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = u[i] * f4_over_one_and_power(g[i], -LOG2E * g[i]);
+  } else if (act == Q3_ACT_GELU_TANH) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = u[i] * f4_over_one_and_power(g[i], g[i] * fmaf(-LOG2E * Z * 0.044715f * g[i], g[i], -LOG2E * Z));
+  } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) a[i] = fmaxf(g[i], 0.f) * u[i];
-    return;
   }
-  const float cubic = act == Q3_ACT_GELU_TANH ? 0.044715f : 0.f, slope = act == Q3_ACT_GELU_TANH ? 1.5957691216057308f : 1.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) a[i] = u[i] * __fdividef(g[i], 1.0f + __expf(-slope * g[i] * fmaf(cubic * g[i], g[i], 1.0f)));
 }
 
 // 64 float32 columns as bfloat16, two to a word.
@@ -254,12 +264,14 @@ __device__ __forceinline__ void f4_gated_block(const uint32_t (&v0)[32], const u
     up[i] = __uint_as_float(c < 32 ? v0[(c + 8) % 32] : v1[(c + 8) % 32]);
   }
   f4_gate<32>(gate, up, p.act, a);
+  if (j * 32 + 32 > inner) {  // uniform over the warp
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (j * 32 + i >= inner) a[i] = 0.f;
+  }
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    if (j * 32 + i >= inner) a[i] = 0.f;
-    top = max(top, __float_as_uint(a[i]) & 0x7fffffffu);
-  }
+  for (int i = 0; i < 32; ++i) top = fp4_top(top, a[i]);
   const uint32_t byte = fp4_scale_byte(top);
   const float inv = fp4_inverse_scale(byte);
   uint32_t w[4];
@@ -556,7 +568,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       for (int i = 0; i < 2; ++i)
         if (block * 32 + place * 2 + i >= inner) a[i] = 0.f;
       const uint32_t half = lane < 16 ? 0xffffu : 0xffff0000u;
-      const uint32_t top = __reduce_max_sync(half, max(__float_as_uint(a[0]) & 0x7fffffffu, __float_as_uint(a[1]) & 0x7fffffffu));
+      const uint32_t top = __reduce_max_sync(half, fp4_top(fp4_top(0u, a[0]), a[1]));
       const uint32_t byte = fp4_scale_byte(top);
       const float inv = fp4_inverse_scale(byte);
       uint32_t c = byte == 255u ? 0u : fp4_pack2(a[0] * inv, a[1] * inv) << (8 * (place & 3));
