@@ -298,7 +298,9 @@ __device__ __forceinline__ void f4_gated_block(const uint32_t (&v0)[32], const u
 //
 // The blocks of a cluster send each row of sums, by asynchronous stores that the receiver's mbarrier counts, to the block that
 // finishes that row (rank r % split).  No block reads another's memory, so none has to stay for the others: a barrier of the
-// whole cluster behind the reading took 1.1 us.  The stores take some two clocks per 16 bytes, so many rows are not shared out.
+// whole cluster behind the reading took 1.1 us.  The stores take some two clocks per 16 bytes; above 8,000 results of a tile a row goes as one
+// bulk copy from shared memory instead, and the blocks stay for each other (by then with an arrival that waits for no stores):
+// 128 x 4,096 x 12,288 11.8 us by stores and 10.2 by copies, 64 rows 9.2 and 8.5, but 64 x 4,096 x 4,096 in tiles of 64 6.1 and 6.4.
 // Twelve warps, four for each 64 columns of a tile: with six in all 8 x 24,576 x 4,096 took 12.35 us instead of 12.1, with a gate and
 // 64 rows 16.2 instead of 14.3.
 constexpr int F4_FEW_THREADS = 384;
@@ -307,11 +309,13 @@ constexpr int F4_FEW_MAX_STAGES = 24;
 constexpr int F4_FEW_MAX_SPLIT = 8;
 constexpr int F4_FEW_COLS = 256;  // tensor memory: up to 192 columns of sums, two times 24 of scales
 constexpr int F4_FEW_SCALE_COLS = 24;
+constexpr int F4_BULK_FROM = 8000;  // results of a tile above which its sums travel by bulk copies
 
 struct F4FewShape {
   int a_rows, bn, stages, split;  // rows of x in a tile (a multiple of 8, at most 128), rows of w in it, stages of the ring, blocks
   int depth;                      // stages that a block works through (the last one of a cluster may have fewer)
   int split_inverse;              // 65536 / split, rounded up: (r * split_inverse) >> 16 = r / split for r < 128
+  int bulk;                       // rows of sums go to the blocks that finish them by bulk copies, else by stores (split > 1)
   int slots;                      // rows of sums that a block of the cluster receives from each (split > 1)
   __host__ __device__ int a_bytes() const { return a_rows * 128; }
   __host__ __device__ int b_bytes() const { return bn * 128; }
@@ -332,6 +336,20 @@ __device__ __forceinline__ uint32_t cluster_id() {
 __device__ __forceinline__ void st_async_v4(uint32_t address, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t bar) {
   asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
                ::"r"(address), "r"(a), "r"(b), "r"(c), "r"(d), "r"(bar)
+               : "memory");
+}
+
+// One of four barriers (`which`, the same in a warp) for `threads` of the block.
+__device__ __forceinline__ void named_barrier(int which, int threads) {
+  if (which == 0) asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
+  else if (which == 1) asm volatile("bar.sync 2, %0;" ::"r"(threads) : "memory");
+  else if (which == 2) asm volatile("bar.sync 3, %0;" ::"r"(threads) : "memory");
+  else asm volatile("bar.sync 4, %0;" ::"r"(threads) : "memory");
+}
+// `bytes` of this block's shared memory to `address` of the cluster's window; the mbarrier at `bar`, in the same block, counts them.
+__device__ __forceinline__ void bulk_to_cluster(uint32_t address, const void* from, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(address), "r"(s_addr(from)), "r"(bytes), "r"(bar)
                : "memory");
 }
 
@@ -487,11 +505,13 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   // Every thread gets here, whatever was given up, so the cluster's barrier needs no bound.
   if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   float* const sums = split > 1 ? received : reinterpret_cast<float*>(smem_raw);  // alone: over the ring, which nothing reads by then
+  const bool by_bulk = shape.bulk != 0;
   // Four warps for each 64 columns of the accumulator, the first of them the last ones: by then they are done with their own work.
   const int c0 = (F4_FEW_THREADS / 128 - 1 - (warp >> 2)) * 64;
   if (c0 < bn && aligned) {
     const int quarter = warp & 3, row = quarter * 32 + lane;
-    if (!warp_wait(acc_full, 0, &abort_flag)) {
+    const bool summed = warp_wait(acc_full, 0, &abort_flag);
+    if (!summed) {
       if (lane == 0) {
         abort_flag = 1;
         atomicOr(status, Q3_STATUS_TIMEOUT);
@@ -507,7 +527,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       if (row >= rows_here) {
       } else if (EPI == 2 && by_rows) {
         if (n0 + c0 < p.N) f4_gated_block(v[0], v[1], p, m0 + row, n0 + c0);
-      } else if (split > 1) {
+      } else if (split > 1 && !by_bulk) {
         const int slot = (row * shape.split_inverse) >> 16, owner = row - slot * split;  // row / split, row % split
         const uint32_t to = cluster_addr(s_addr(received + (rank * shape.slots + slot) * bn), owner);
         const uint32_t bar = cluster_addr(s_addr(sums_full), owner);
@@ -518,8 +538,18 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       } else {  // rows bn + 4 values apart, off each other's banks
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          *reinterpret_cast<uint4*>(sums + row * (bn + 4) + c0 + 4 * j) =
+          *reinterpret_cast<uint4*>(reinterpret_cast<float*>(smem_raw) + row * (bn + 4) + c0 + 4 * j) =
               make_uint4(v[j / 8][4 * (j % 8)], v[j / 8][4 * (j % 8) + 1], v[j / 8][4 * (j % 8) + 2], v[j / 8][4 * (j % 8) + 3]);
+      }
+      __syncwarp();
+    }
+    if (by_bulk && quarter * 32 < rows_here) {
+      fence_async_proxy();  // the copies read what these stores left
+      named_barrier(quarter, bn / 2);  // of the warps of these 32 rows, all of which get here
+      if (summed && c0 == 0 && row < rows_here) {
+        const int slot = (row * shape.split_inverse) >> 16, owner = row - slot * split;
+        bulk_to_cluster(cluster_addr(s_addr(received + (rank * shape.slots + slot) * bn), owner),
+                        reinterpret_cast<float*>(smem_raw) + row * (bn + 4), bn * 4, cluster_addr(s_addr(sums_full), owner));
       }
       __syncwarp();
     }
@@ -533,15 +563,16 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   }
   // A block that gave up does not cut this wait short: the others' sums may still be on their way into its memory.
   int never = 0;
-  if (split > 1 && !warp_wait(sums_full, 0, &never)) {
-    if (lane == 0) atomicOr(status, Q3_STATUS_TIMEOUT);
-    return;
-  }
+  const bool here = split == 1 || warp_wait(sums_full, 0, &never);
+  if (!here && lane == 0) atomicOr(status, Q3_STATUS_TIMEOUT);
+  __syncwarp();
+  // What was sent by bulk copies is read from here until it is there: a block stays until all of its cluster have their sums.
+  if (by_bulk) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   // Sixteen lanes finish 64 columns of a row, four to a lane.  The blocks' sums are added in the order of their ranges of k.
   const int inner = p.N / 2, out_across = fp4_tiles(inner), blocks = (inner + FP4_BLOCK - 1) / FP4_BLOCK;
   const int groups = bn / 64, my_rows = ((rows_here - rank + split - 1) * shape.split_inverse) >> 16;
-  const int items = by_rows ? 0 : my_rows * groups, l = lane & 15;
+  const int items = by_rows || !here ? 0 : my_rows * groups, l = lane & 15;
   for (int i0 = warp * 2; i0 < items; i0 += 2 * (F4_FEW_THREADS / 32)) {
     const int item = min(i0 + (lane >> 4), items - 1);  // lanes without an item of their own do the last one again
     const int slot = groups == 1 ? item : groups == 2 ? item >> 1 : item / 3, g = item - slot * groups;
@@ -606,6 +637,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       }
     }
   }
+  if (by_bulk) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ---------------------------------------------------------------- many tokens: tiles of 256 x 192, 256 or 384 by pairs of CTAs
@@ -990,11 +1022,12 @@ static F4FewShape f4_few_shape(int T, int N, int K, double* clocks) {
   const int k_stages = (fp4_tiles(K) + 1) / 2, rows = T < F4_BM ? T : F4_BM, *const slots = f4_few_slots();
   for (int bn = 64; bn <= 192; bn += 64) {
     const long long tiles = (long long)((N + bn - 1) / bn) * ((T + F4_BM - 1) / F4_BM);
+    const int results = rows * bn, sums = results > F4_BULK_FROM && results <= 128 * 160 ? 3000 + results / 5 : 600 + results / 2;
     for (int split = 1; split <= F4_FEW_MAX_SPLIT && split <= k_stages; ++split) {
       const int depth = (k_stages + split - 1) / split;
       if ((split - 1) * depth >= k_stages) continue;  // no block without a stage
       const double rounds = (double)((tiles + slots[split] - 1) / slots[split]);
-      const double cost = rounds * (depth * (bn == 64 ? 386 : bn == 128 ? 415 : 470) + (split > 1 ? 600 + rows * bn / 2 : 0));
+      const double cost = rounds * (depth * (bn == 64 ? 386 : bn == 128 ? 415 : 470) + (split > 1 ? sums : 0));
       if (best.bn == 0 || cost < best_cost) {
         best_cost = cost;
         best_rounds = rounds;
@@ -1020,6 +1053,7 @@ static F4FewShape f4_few_shape(int T, int N, int K, double* clocks) {
     if (room > 160 * 1024 || ((best.stages >= 3 || best.stages == best.depth) && best.ring_bytes() >= alone)) break;
   }
   while (best.ring_bytes() < alone) ++best.stages;
+  best.bulk = best.split > 1 && rows * best.bn > F4_BULK_FROM && rows * (best.bn + 4) * 4 <= best.ring_bytes();
   // Rounds of blocks that take more than half of an SM's shared memory do not overlap (128 rows of 192 columns: some 8,000 clocks from
   // one's start to its first stage and from its last one to its end).
   const double apart = best.smem_bytes() > 113 * 1024 ? (best_rounds - 1) * (3000 + rows * best.bn / 5) : 0;
