@@ -345,8 +345,9 @@ def dtype_tag(dtype: torch.dtype) -> int:
 
 
 def _stream() -> int:
-    """The handle of torch's current stream (asked for without a Stream object around it: 0.3 us a call instead of 3.1)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    """The handle of torch's current stream on the current device, asked for after tensors on a GPU have been seen (without a Stream
+    object around it and without asking whether CUDA is set up: 0.1 us a call instead of 3.1)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -105,6 +105,22 @@ def test_quantise_ties_ends_and_signs():
     assert int(b.scales.reshape(-1)[0]) == 253 and bool((b.codes == 0x66).all())
 
 
+@pytest.mark.parametrize("out", list(DT))
+@pytest.mark.parametrize("width", [1, 7, 9, 255, 257, 263, 1023, 1025, 1031, 2049, 2300])
+def test_quantise_values_off_every_boundary(width, out):
+    """Values whose rows begin at every place within 16 bytes: those that the codes stand for, and nothing around them is touched."""
+    x = normal(18, width, width)
+    own = ops().fp4_rows(18, width, "cuda")
+    ops().fp4_quantise(x.cuda(), own)
+    want, _ = plain.read(own.codes, own.scales, width)
+    for start in range(0, 9):
+        room = torch.full((18 * width + 64,), 3.0, dtype=DT[out], device="cuda")
+        values = room[start:start + 18 * width].view(18, width)
+        ops().fp4_quantise(x.cuda(), ops().fp4_rows(18, width, "cuda"), values)
+        assert torch.equal(values.cpu().double(), want), start
+        assert bool((room[:start] == 3).all()) and bool((room[start + 18 * width:] == 3).all()), start
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_quantise_what_is_not_finite(bad):
     x = normal(3, 100, 5)
