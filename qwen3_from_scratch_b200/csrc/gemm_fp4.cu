@@ -291,8 +291,8 @@ __device__ __forceinline__ void f4_gated_block(const uint32_t (&v0)[32], const u
 
 // ---------------------------------------------------------------- a few tokens: small tiles, k shared out
 // A tile is up to 128 rows of x by 64, 128 or 192 rows of w, and `split` blocks of a cluster share out its range of k.  What
-// bounds it is w's bytes where w is large (8 x 24,576 x 4,096: 12.4 us, 4.3 TB/s between the start of one call and of the next, some
-// 5.7 while w streams) and the chain of latencies between two kernels where it is not (64 x 4,096 x 4,096: 6.2 us for 1.5 us of
+// bounds it is w's bytes where w is large (8 x 24,576 x 4,096: 12.1 to 12.5 us, 4.3 TB/s between the start of one call and of the next, some
+// 5.7 while w streams) and the chain of latencies between two kernels where it is not (64 x 4,096 x 4,096: 5.9 us for 1.5 us of
 // bytes: 1 from the kernel before to this one's start, 1 for x, 1 for the main loop, 2 for the sums and the results), so the sizes
 // are chosen (f4_few_shape) to give each SM one block.
 //

@@ -571,6 +571,30 @@ def test_a_wait_that_runs_out_is_given_up_cleanly(rows, features, width, form):
     assert bool(((y.cpu().double() - want).abs() <= product_tolerance(xv, wv) + want.abs() * 2.0 ** -8).all())
 
 
+@pytest.mark.parametrize("drop", [0, 1])
+@pytest.mark.parametrize("rows,features,width", [(100, 512, 12288), (128, 1000, 4352), (70, 300, 2304), (200, 130, 8448)])
+def test_sums_by_copies_are_given_up_cleanly(rows, features, width, drop):
+    """Tiles whose sums go from block to block as copies, where all blocks give up or all but those with a single stage."""
+    o = ops()
+    x, xv = held(normal(rows, width, 1))
+    w, wv = held(normal(features, width, 2, False))
+    y, st = torch.empty(rows, features, device="cuda", dtype=torch.bfloat16), status()
+    try:
+        o.set_wait_test(limit=1 << 14, drop_copy=drop)
+        o.fp4_product(x, w, y, st, form="few")
+        torch.cuda.synchronize()
+        word = int(st.item())
+    finally:
+        o.set_wait_test()
+    assert word & 16, f"status {word}: the time-out bit is not set"
+    st.zero_()
+    want = xv @ wv.t()
+    for _ in range(3):
+        o.fp4_product(x, w, y, st, form="few")
+        assert int(st.item()) == 0
+        assert bool(((y.cpu().double() - want).abs() <= product_tolerance(xv, wv) + want.abs() * 2.0 ** -8).all())
+
+
 # ---------------------------------------------------------------- a model whose feed-forwards are held so
 def plain_mlp(x, w, prefix):
     """The feed-forward of the plain model with weights and activations rounded."""
