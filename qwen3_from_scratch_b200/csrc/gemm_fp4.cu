@@ -133,7 +133,7 @@ struct F4RowStore {
   __device__ __forceinline__ F4RowStore(const F4Args& p, unsigned char* stage_, int row0, int col, int cols)
       : stage(stage_), first((unsigned char*)p.out + ((size_t)row0 * p.ldc + col) * sizeof(OutT)), pitch((size_t)p.ldc * sizeof(OutT)),
         rows(min(32, p.T - row0)), bytes(min(cols, p.N - col) * (int)sizeof(OutT)), at(0),
-        whole(col + cols <= p.N && (((uintptr_t)p.out | (size_t)p.ldc * sizeof(OutT)) & 31) == 0) {}
+        whole(col + cols <= p.N && (((uintptr_t)p.out | (size_t)p.ldc * sizeof(OutT)) & 31) == 0), held{} {}
 
   // The next 128 bytes of each row.
   __device__ __forceinline__ void push(const uint32_t (&w)[32], int lane) {
@@ -178,12 +178,15 @@ struct F4RowStore {
   }
 
  private:
-  __device__ __forceinline__ uint4 piece(int r, int c) const { return *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4)); }
+  __device__ __forceinline__ uint4 piece(int r, int c) const {
+    return *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
+  }
   __device__ __forceinline__ void put(const uint32_t (&y)[32], int lane, int pieces) {
 #pragma unroll
     for (int c = 0; c < 8; ++c)
       if (c < pieces)
-        *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
+        *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+            make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
     __syncwarp();
   }
   // x, from its ninth word on, moves up by as many bytes as the lane's row is behind a sector's boundary.
@@ -298,9 +301,10 @@ __device__ __forceinline__ void f4_gated_block(const uint32_t (&v0)[32], const u
 //
 // The blocks of a cluster send each row of sums, by asynchronous stores that the receiver's mbarrier counts, to the block that
 // finishes that row (rank r % split).  No block reads another's memory, so none has to stay for the others: a barrier of the
-// whole cluster behind the reading took 1.1 us.  The stores take some two clocks per 16 bytes; above 8,000 results of a tile a row goes as one
-// bulk copy from shared memory instead, and the blocks stay for each other (by then with an arrival that waits for no stores):
-// 128 x 4,096 x 12,288 11.8 us by stores and 10.2 by copies, 64 rows 9.2 and 8.5, but 64 x 4,096 x 4,096 in tiles of 64 6.1 and 6.4.
+// whole cluster behind the reading took 1.1 us.  The stores take some two clocks per 16 bytes; above 8,000 results of a tile a row
+// goes as one bulk copy from shared memory instead, and the blocks stay for each other (by then with an arrival that waits for no
+// stores): 128 x 4,096 x 12,288 11.8 us by stores and 10.2 by copies, 64 rows 9.2 and 8.5, but 64 x 4,096 x 4,096 in tiles of 64
+// 6.1 and 6.4.
 // Twelve warps, four for each 64 columns of a tile: with six in all 8 x 24,576 x 4,096 took 12.35 us instead of 12.1, with a gate and
 // 64 rows 16.2 instead of 14.3.
 constexpr int F4_FEW_THREADS = 384;
@@ -321,7 +325,8 @@ struct F4FewShape {
   __host__ __device__ int b_bytes() const { return bn * 128; }
   __host__ __device__ int w_scale_tiles() const { return (bn + FP4_TILE - 1) / FP4_TILE; }
   __host__ __device__ int stage_bytes() const { return a_bytes() + b_bytes() + (1 + w_scale_tiles()) * 2 * FP4_TILE_BYTES; }
-  __host__ __device__ int behind_bytes() const { return 128 * 128 > stage_bytes() ? 128 * 128 - stage_bytes() : 0; }  // the last x tile is read as 128 rows
+  // the last x tile is read as 128 rows
+  __host__ __device__ int behind_bytes() const { return 128 * 128 > stage_bytes() ? 128 * 128 - stage_bytes() : 0; }
   __host__ __device__ int ring_bytes() const { return stages * stage_bytes() + behind_bytes(); }
   __host__ __device__ int received_bytes() const { return split > 1 ? split * slots * bn * 4 : 0; }
   __host__ __device__ size_t smem_bytes() const { return (size_t)ring_bytes() + received_bytes() + F4_BAR_BYTES; }
