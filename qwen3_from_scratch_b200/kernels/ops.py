@@ -3154,7 +3154,10 @@ class Fp4Rows(NamedTuple):
 
     ``codes``: uint8 [rows, 16 ceil(width / 32)], value 2 i in the low half of byte i; zeros beyond the width.
     ``scales``: uint8, tiles of 128 rows x 4 blocks, [at least ceil(rows / 128), ceil(width / 128), 512]: the byte b of row r,
-    block j is byte 16 (r % 32) + 4 ((r % 128) / 32) + j % 4 of tile (r / 128, j / 4); zeros beyond the width.  255 is NaN."""
+    block j is byte 16 (r % 32) + 4 ((r % 128) / 32) + j % 4 of tile (r / 128, j / 4); zeros beyond the width.  255 is NaN.
+
+    The products read rows whose bytes lie in int16, int32 or int64 as well, at the cost of a pass that narrows them in every call;
+    rows that a call writes are uint8."""
 
     codes: torch.Tensor
     scales: torch.Tensor
@@ -3190,6 +3193,19 @@ def _check_fp4(name: str, r: Fp4Rows, width: Optional[int] = None, rows: Optiona
     if (width is not None and k != width) or (rows is not None and size[0] != rows):
         raise KernelError(f"{name}: {size[0]} rows of {k} values, expected {size[0] if rows is None else rows} of "
                           f"{k if width is None else width}")
+
+
+_FP4_WIDER = (torch.int16, torch.int32, torch.int64)
+
+
+def _fp4_bytes(r: Fp4Rows) -> Fp4Rows:
+    """Rows that a call reads.  Arithmetic on bytes in torch ends in a wider integer type as soon as one operand is one; codes or scales
+    that lie so are narrowed to the bytes that they hold, in memory that lasts until the call's kernels have run."""
+    codes, scales = r.codes, r.scales
+    if codes.dtype is scales.dtype is torch.uint8:
+        return r
+    return Fp4Rows(codes.to(torch.uint8) if codes.dtype in _FP4_WIDER else codes,
+                   scales.to(torch.uint8) if scales.dtype in _FP4_WIDER else scales, r.width)
 
 
 def fp4_quantise(x: torch.Tensor, out: Fp4Rows, values: Optional[torch.Tensor] = None) -> None:
@@ -3259,6 +3275,7 @@ def fp4_product(x: Fp4Rows, w: Fp4Rows, out: torch.Tensor, status: torch.Tensor,
     """out[T, N] = x[T, K] @ w[N, K]^T of rows held in four bits, accumulated in float32; out bfloat16 or float32, also a column
     view of a wider buffer.  ``form``: one of ``FP4_FORMS`` instead of the one that the sizes ask for (a few tokens' small tiles,
     or tiles of that many columns by pairs of CTAs, 384 for bfloat16 results only)."""
+    x, w = _fp4_bytes(x), _fp4_bytes(w)
     _check_fp4("fp4_product.x", x)
     _check_fp4("fp4_product.w", w, x.width)
     T, N = x.codes.shape[0], w.codes.shape[0]
@@ -3284,6 +3301,7 @@ def fp4_gated_product(x: Fp4Rows, w: Fp4Rows, out: Fp4Rows, status: torch.Tensor
                       form: Optional[str] = None) -> None:
     """out = the rows of act(gate) * up, rounded as by ``fp4_quantise`` from float32: w's 2 I rows alternate gate/up in blocks
     of eight (I a multiple of 8), gate and up are the products of x with them.  ``form``: see ``fp4_product``."""
+    x, w = _fp4_bytes(x), _fp4_bytes(w)
     _check_fp4("fp4_gated_product.x", x)
     _check_fp4("fp4_gated_product.w", w, x.width)
     _check_fp4("fp4_gated_product.out", out, w.rows // 2, x.rows)
@@ -3302,6 +3320,7 @@ def fp4_feed_forward(stream: torch.Tensor, delta: Optional[torch.Tensor], weight
     with ``gate_up`` [2 I, H] into ``gated`` [T, I], and out[T, H] = gated @ down[H, I]^T; delta has the dtype of out."""
     size = T, H = _check_fp4_stream("fp4_feed_forward", stream, delta, weight, stream_out, out.dtype)
     _check_rows("fp4_feed_forward.out", out, out.dtype, size)
+    gate_up, down = _fp4_bytes(gate_up), _fp4_bytes(down)
     inner = down.width
     _check_fp4("fp4_feed_forward.gate_up", gate_up, H, 2 * inner)
     _check_fp4("fp4_feed_forward.down", down, inner, H)

@@ -32,3 +32,18 @@ def test_tensors_off_the_gpu_are_refused():
         ops.fp4_product(r, r, torch.zeros(2, 2), torch.zeros(1, dtype=torch.int32))
     with pytest.raises(ops.KernelSizeError):
         ops.fp4_rows(-1, 64, "cpu")
+
+
+@pytest.mark.parametrize("wide", [torch.int16, torch.int32, torch.int64])
+def test_bytes_in_a_wider_integer_type_are_read_as_bytes(wide):
+    from qwen3_from_scratch_b200.kernels import ops
+    codes = torch.arange(256, dtype=torch.uint8).view(8, 32)
+    scales = (torch.arange(512) % 256).to(torch.uint8).view(1, 1, 512)
+    for c, s in ((codes.to(wide), scales), (codes, scales.to(wide)), (codes.to(wide), scales.to(wide))):
+        r = ops._fp4_bytes(ops.Fp4Rows(c, s, 64))
+        assert r.codes.dtype is r.scales.dtype is torch.uint8 and r.width == 64
+        assert torch.equal(r.codes, codes) and torch.equal(r.scales, scales)
+    own = ops.Fp4Rows(codes, scales, 64)
+    assert ops._fp4_bytes(own) is own
+    other = ops.Fp4Rows(codes.float(), scales, 64)
+    assert ops._fp4_bytes(other).codes.dtype is torch.float32

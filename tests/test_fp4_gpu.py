@@ -640,3 +640,33 @@ def test_engine_generates_with_fp4_feed_forwards(tiny_folders):
     assert first == again and [len(t) for t in first] == [12, 12]
     with pytest.raises(ValueError, match="fp4"):
         SyncEngine(tiny_folders["d"], num_pages=64, feed_forward_weights="int3")
+
+
+# ---------------------------------------------------------------- codes and scales as arithmetic on bytes leaves them
+@pytest.mark.parametrize("wide", [torch.int16, torch.int32, torch.int64])
+@pytest.mark.parametrize("rows,inner,width", [(3, 40, 264), (300, 72, 128)])
+def test_products_of_bytes_in_a_wider_integer_type(rows, inner, width, wide):
+    o = ops()
+    x, gu = held(normal(rows, width, 1))[0], held(interleaved(normal(inner, width, 2, False), normal(inner, width, 3, False)))[0]
+    down = held(normal(width, inner, 4, False))[0]
+    as_wide = [o.Fp4Rows(r.codes.to(wide), r.scales.to(wide), r.width) for r in (x, gu, down)]
+    st, y, y2 = status(), torch.empty(rows, 2 * inner, device="cuda"), torch.empty(rows, 2 * inner, device="cuda")
+    o.fp4_product(x, gu, y, st)
+    o.fp4_product(as_wide[0], as_wide[1], y2, st)
+    assert torch.equal(y, y2)
+    a, a2 = o.fp4_rows(rows, inner, "cuda"), o.fp4_rows(rows, inner, "cuda")
+    o.fp4_gated_product(x, gu, a, st)
+    o.fp4_gated_product(as_wide[0], as_wide[1], a2, st)
+    assert torch.equal(a.codes, a2.codes)
+    stream, norm, h = normal(rows, width, 5).cuda(), torch.ones(width, device="cuda"), o.fp4_rows(rows, width, "cuda")
+    z, z2 = torch.empty(rows, width, device="cuda"), torch.empty(rows, width, device="cuda")
+    o.fp4_feed_forward(stream, None, norm, 1e-6, gu, down, h, a, z, st)
+    o.fp4_feed_forward(stream, None, norm, 1e-6, as_wide[1], as_wide[2], h, a2, z2, st)
+    assert torch.equal(z, z2) and int(st.item()) == 0
+    # what a call writes has to be bytes, and what it reads has to be whole numbers
+    with pytest.raises(o.KernelError, match="uint8"):
+        o.fp4_quantise(stream, o.Fp4Rows(h.codes.to(wide), h.scales, width))
+    with pytest.raises(o.KernelError, match="uint8"):
+        o.fp4_gated_product(x, gu, o.Fp4Rows(a.codes.to(wide), a.scales, inner), st)
+    with pytest.raises(o.KernelError, match="uint8"):
+        o.fp4_product(o.Fp4Rows(x.codes.float(), x.scales, width), gu, y, st)
