@@ -372,7 +372,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   uint64_t* acc_full = empty + stages;
   uint64_t* sums_full = acc_full + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sums_full + 1);
-  __shared__ int abort_flag;
+  __shared__ int abort_flag, stay;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = split > 1 ? (int)cluster_rank() : 0, tile = split > 1 ? (int)cluster_id() : blockIdx.x;
@@ -402,6 +402,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   };
   if (threadIdx.x == 0) {
     abort_flag = 0;
+    stay = 0;  // set by a block of the cluster whose wait for its sums runs out (sums by bulk copies)
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -413,7 +414,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     if (split > 1) mbar_expect_tx(sums_full, (uint32_t)(split * (((rows_here - rank + split - 1) * shape.split_inverse) >> 16) * bn * 4));
   }
   __syncthreads();
-  if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // waited for before anything is sent
+  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for before anything is sent
 
   if (warp == 0) {
     // Where w is known not to come from the kernel before, its part of the ring's first round goes out ahead of the wait.
@@ -571,8 +572,23 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   const bool here = split == 1 || warp_wait(sums_full, 0, &never);
   if (!here && lane == 0) atomicOr(status, Q3_STATUS_TIMEOUT);
   __syncwarp();
-  // What was sent by bulk copies is read from here until it is there: a block stays until all of its cluster have their sums.
-  if (by_bulk) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if (by_bulk) {
+    // What was sent by bulk copies is read from here until it is there: a block stays until all of its cluster have their sums, or,
+    // where one's wait ran out, until that one says so and the copies have had another such wait (below).
+    if (here) {
+      asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    } else {
+      if (lane < split) st_cluster_u32(cluster_addr(s_addr(&stay), lane), 1u);  // none of them leaves before this warp arrives
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    }
+  } else if (!here) {
+    // Another block may be late by several waits of its own and send its sums only now.  So this warp stays until every thread of the
+    // cluster has sent all that it will (one that has returned holds the barrier up no longer, so the others wait for nobody), and
+    // then for what is still on its way.
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    warp_wait(sums_full, 0, &never);
+  }
 
   // Sixteen lanes finish 64 columns of a row, four to a lane.  The blocks' sums are added in the order of their ranges of k.
   const int inner = p.N / 2, out_across = fp4_tiles(inner), blocks = (inner + FP4_BLOCK - 1) / FP4_BLOCK;
@@ -642,7 +658,13 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       }
     }
   }
-  if (by_bulk) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (by_bulk) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (*(volatile int*)&stay) {  // the same in every thread of the cluster: written before the barrier or not at all
+      warp_wait(sums_full, 0, &never);
+      asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+  }
 }
 
 // ---------------------------------------------------------------- many tokens: tiles of 256 x 192, 256 or 384 by pairs of CTAs

@@ -595,6 +595,35 @@ def test_sums_by_copies_are_given_up_cleanly(rows, features, width, drop):
         assert bool(((y.cpu().double() - want).abs() <= product_tolerance(xv, wv) + want.abs() * 2.0 ** -8).all())
 
 
+@pytest.mark.parametrize("drop", [0, 1])
+@pytest.mark.parametrize("rows,features,width", [(1, 200, 2816), (3, 200, 2816), (20, 136, 2816), (30, 48, 4352)])
+def test_sums_by_stores_are_given_up_cleanly(rows, features, width, drop):
+    """Tiles whose sums go from block to block as stores, where all blocks give up or all but one of a single stage, which sends its
+    sums to blocks that wait for more and waits itself for what never comes."""
+    o = ops()
+    x, xv = held(normal(rows, width, 1))
+    w, wv = held(normal(features, width, 2, False))
+    y, a, st = torch.empty(rows, features, device="cuda"), o.fp4_rows(rows, features // 2, "cuda"), status()
+    for call in (lambda: o.fp4_product(x, w, y, st, form="few"), lambda: o.fp4_gated_product(x, w, a, st, form="few")):
+        try:
+            o.set_wait_test(limit=1 << 14, drop_copy=drop)
+            call()
+            torch.cuda.synchronize()
+            word = int(st.item())
+        finally:
+            o.set_wait_test()
+        assert word & 16, f"status {word}: the time-out bit is not set"
+        st.zero_()
+    want, first = xv @ wv.t(), None
+    for _ in range(3):
+        o.fp4_product(x, w, y, st, form="few")
+        o.fp4_gated_product(x, w, a, st, form="few")
+        assert int(st.item()) == 0
+        assert bool(((y.cpu().double() - want).abs() <= product_tolerance(xv, wv)).all())
+        first = a.codes.clone() if first is None else first
+        assert torch.equal(a.codes, first)
+
+
 # ---------------------------------------------------------------- a model whose feed-forwards are held so
 def plain_mlp(x, w, prefix):
     """The feed-forward of the plain model with weights and activations rounded."""
