@@ -567,9 +567,10 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(F4_FEW_COLS) : "memory");
   }
-  // A block that gave up does not cut this wait short: the others' sums may still be on their way into its memory.
+  // A block that gave up does not cut this wait short: the others' sums may still be on their way into its memory.  What other blocks
+  // wrote is acquired at the cluster's scope.
   int never = 0;
-  const bool here = split == 1 || warp_wait(sums_full, 0, &never);
+  const bool here = split == 1 || warp_wait_cluster(sums_full, 0, &never);
   if (!here && lane == 0) atomicOr(status, Q3_STATUS_TIMEOUT);
   __syncwarp();
   if (by_bulk) {
@@ -587,7 +588,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     // cluster has sent all that it will (one that has returned holds the barrier up no longer, so the others wait for nobody), and
     // then for what is still on its way.
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    warp_wait(sums_full, 0, &never);
+    warp_wait_cluster(sums_full, 0, &never);
   }
 
   // Sixteen lanes finish 64 columns of a row, four to a lane.  The blocks' sums are added in the order of their ranges of k.
@@ -661,7 +662,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   if (by_bulk) {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (*(volatile int*)&stay) {  // the same in every thread of the cluster: written before the barrier or not at all
-      warp_wait(sums_full, 0, &never);
+      warp_wait_cluster(sums_full, 0, &never);
       asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
   }
