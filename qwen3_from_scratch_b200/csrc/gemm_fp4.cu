@@ -1197,11 +1197,22 @@ static bool f4_aligned(const void* a, const void* b, const void* c, const void* 
   return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) & 15) == 0;
 }
 
+// What is asked of a call before anything of it, or of the calls that belong with it, is launched.
+static int fp4_product_check(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, int T, int N, int K,
+                             long long ldc) {
+  if (!f4_sizes_ok(T, N, K) || ldc < N) return Q3_ERR_SIZE;
+  return f4_aligned(x_codes, x_scales, w_codes, w_scales) ? 0 : Q3_ERR_ALIGN;
+}
+static int fp4_gated_check(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, const void* out_codes,
+                           const void* out_scales, int T, int N, int K, int act) {
+  if (!f4_sizes_ok(T, N, K) || N % 16 || (act != Q3_ACT_SILU && act != Q3_ACT_RELU && act != Q3_ACT_GELU_TANH)) return Q3_ERR_SIZE;
+  return f4_aligned(x_codes, x_scales, w_codes, w_scales) && f4_aligned(out_codes, out_scales, nullptr, nullptr) ? 0 : Q3_ERR_ALIGN;
+}
+
 static int fp4_product(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out, int T, int N,
                        int K, long long ldc, int out_f32, int form, int early, int* status, cudaStream_t stream) {
   if (T <= 0) return 0;
-  if (!f4_sizes_ok(T, N, K) || ldc < N) return Q3_ERR_SIZE;
-  if (!f4_aligned(x_codes, x_scales, w_codes, w_scales)) return Q3_ERR_ALIGN;
+  if (const int code = fp4_product_check(x_codes, x_scales, w_codes, w_scales, T, N, K, ldc)) return code;
   const F4Args p{(const uint8_t*)x_scales, (const uint8_t*)w_scales, out, ldc, nullptr, nullptr, T, N, K, 0};
   if (out_f32) return gemm_fp4<1>(x_codes, w_codes, p, form, early, status, stream);
   return gemm_fp4<0>(x_codes, w_codes, p, form, early, status, stream);
@@ -1210,8 +1221,7 @@ static int fp4_product(const void* x_codes, const void* x_scales, const void* w_
 static int fp4_gated_product(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out_codes,
                              void* out_scales, int T, int N, int K, int act, int form, int early, int* status, cudaStream_t stream) {
   if (T <= 0) return 0;
-  if (!f4_sizes_ok(T, N, K) || N % 16 || (act != Q3_ACT_SILU && act != Q3_ACT_RELU && act != Q3_ACT_GELU_TANH)) return Q3_ERR_SIZE;
-  if (!f4_aligned(x_codes, x_scales, w_codes, w_scales) || !f4_aligned(out_codes, out_scales, nullptr, nullptr)) return Q3_ERR_ALIGN;
+  if (const int code = fp4_gated_check(x_codes, x_scales, w_codes, w_scales, out_codes, out_scales, T, N, K, act)) return code;
   const F4Args p{(const uint8_t*)x_scales, (const uint8_t*)w_scales, nullptr, 0, (uint8_t*)out_codes, (uint8_t*)out_scales, T, N, K, act};
   return gemm_fp4<2>(x_codes, w_codes, p, form, early, status, stream);
 }
@@ -1237,12 +1247,18 @@ extern "C" int q3_fp4_gated_product(const void* x_codes, const void* x_scales, c
 // A gated feed-forward behind its norm, in three launches: the norm's rows into h, the gated product into a, y = a w_down^T.  What
 // runs before each product is the launch above it here, which writes neither product's w, so both may read theirs ahead of it; all
 // that ran before this call is over when the norm's kernel lets the next one start.  (Before a product called by itself anything
-// may have run, the kernel that writes its w included; there reading ahead gains nothing that could be measured.)
+// may have run, the kernel that writes its w included; there reading ahead gains nothing that could be measured.)  All three are
+// checked before the first is launched: the norm may update the stream in place, and a call that refuses leaves it as it was.
 extern "C" int q3_fp4_feed_forward(const float* stream_in, const void* delta, const float* norm, float* stream_out, float eps,
                                    const void* gu_codes, const void* gu_scales, const void* down_codes, const void* down_scales,
                                    void* h_codes, void* h_scales, void* a_codes, void* a_scales, void* y, int dtype, int T,
                                    int H, int I, int act, int* status, cudaStream_t stream) {
-  int code = q3_fp4_add_rmsnorm(stream_in, delta, dtype, norm, stream_out, h_codes, h_scales, T, H, eps, stream);
+  if (T <= 0) return 0;
+  if (I <= 0 || I > (1 << 29)) return Q3_ERR_SIZE;
+  int code = q3::fp4_gated_check(h_codes, h_scales, gu_codes, gu_scales, a_codes, a_scales, T, 2 * I, H, act);
+  if (!code) code = q3::fp4_product_check(a_codes, a_scales, down_codes, down_scales, T, H, I, H);
+  if (code) return code;
+  code = q3_fp4_add_rmsnorm(stream_in, delta, dtype, norm, stream_out, h_codes, h_scales, T, H, eps, stream);
   if (code) return code;
   code = q3::fp4_gated_product(h_codes, h_scales, gu_codes, gu_scales, a_codes, a_scales, T, 2 * I, H, act, 0, 1, status, stream);
   if (code) return code;

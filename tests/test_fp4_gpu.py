@@ -549,6 +549,41 @@ def test_refusals():
     assert int(st.item()) == 0
 
 
+def test_a_refused_feed_forward_leaves_the_stream_alone():
+    o, rows, width, inner = ops(), 3, 64, 40
+    stream, delta, st = normal(rows, width, 1).cuda(), normal(rows, width, 2).cuda(), status()
+    before, norm, y = stream.clone(), torch.ones(width, device="cuda"), torch.full((rows, width), 7.0, device="cuda")
+
+    def off_by_eight(r):
+        room = torch.zeros(r.codes.numel() + 16, dtype=torch.uint8, device="cuda")
+        return o.Fp4Rows(room[8:8 + r.codes.numel()].view(r.codes.shape), r.scales, r.width)
+
+    def scales_off_by_eight(r):
+        room = torch.zeros(r.scales.numel() + 16, dtype=torch.uint8, device="cuda")
+        return o.Fp4Rows(r.codes, room[8:8 + r.scales.numel()].view(r.scales.shape), r.width)
+
+    def call(i=inner, change=None, which=None, **more):
+        rows4 = [o.fp4_rows(2 * i, width, "cuda"), o.fp4_rows(width, i, "cuda"), o.fp4_rows(rows, width, "cuda"), o.fp4_rows(rows, i, "cuda")]
+        if which is not None:
+            rows4[which] = change(rows4[which])
+        o.fp4_feed_forward(stream, delta, norm, 1e-6, *rows4, y, st, **more)
+
+    with pytest.raises(o.KernelSizeError):
+        call(12)
+    for which in range(4):
+        for change in (off_by_eight, scales_off_by_eight):
+            with pytest.raises(o.KernelError, match="misaligned"):
+                call(change=change, which=which)
+    with pytest.raises(o.KernelError, match="gate"):
+        call(activation="limited")
+    with pytest.raises(o.KernelError, match="expected"):
+        call(change=lambda r: o.fp4_rows(width, inner + 8, "cuda"), which=1)
+    torch.cuda.synchronize()
+    assert torch.equal(stream, before) and bool((y == 7).all()) and int(st.item()) == 0
+    call()
+    assert torch.equal(stream, before + delta)
+
+
 @pytest.mark.parametrize("form", ["few", "pair192", "pair256", "pair384"])
 @pytest.mark.parametrize("rows,features,width", [(3, 200, 3000), (600, 800, 1024)])
 def test_a_wait_that_runs_out_is_given_up_cleanly(rows, features, width, form):
