@@ -98,7 +98,11 @@ __device__ __forceinline__ void f4_gate(const float (&g)[N], const float (&u)[N]
     for (int i = 0; i < N; ++i) a[i] = u[i] * f4_over_one_and_power(g[i], g[i] * fmaf(-LOG2E * Z * 0.044715f * g[i], g[i], -LOG2E * Z));
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) a[i] = fmaxf(g[i], 0.f) * u[i];
+    for (int i = 0; i < N; ++i) {
+      float m;  // a NaN stays one
+      asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(m) : "f"(g[i]));
+      a[i] = m * u[i];
+    }
   }
 }
 

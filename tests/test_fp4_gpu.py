@@ -369,6 +369,22 @@ def test_gated_product_of_what_is_not_finite(rows, form):
     assert bool(torch.isfinite(got[0]).all()) and bool((byte[0] < 255).all())
 
 
+@pytest.mark.parametrize("act", ["silu", "relu", "gelu_tanh"])
+@pytest.mark.parametrize("half", ["gate", "up"])
+@pytest.mark.parametrize("rows,form", [(3, "few"), (3, None), (40, "few"), (260, "few"), (260, "pair192"), (260, "pair256")])
+def test_gated_product_of_one_row_that_is_not_finite(rows, form, half, act):
+    """A NaN in one gate or up row alone: the block of results that holds its column is NaN in every row, no other is."""
+    parts = {"gate": normal(72, 2304, 1, False), "up": normal(72, 2304, 2, False)}
+    parts[half][37, 9] = math.nan
+    x, w = held(normal(rows, 2304, 3))[0], held(interleaved(parts["gate"], parts["up"]))[0]
+    r, st = junk_rows(rows, 72), status()
+    ops().fp4_gated_product(x, w, r, st, activation=act, form=form)
+    got, byte = plain.read(r.codes, r.scales, 72)
+    assert int(st.item()) == 0
+    assert bool((byte[:, 1] == 255).all()) and bool((byte[:, [0, 2]] < 255).all())
+    assert bool(torch.isnan(got[:, 32:64]).all()) and bool(torch.isfinite(got[:, :32]).all())
+
+
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("rows,width,inner", [(1, 8, 8), (1, 256, 520), (1, 4096, 1200), (3, 4104, 200), (7, 8192 // 2, 328), (24, 512, 1000), (24, 1000, 504),
                                               (32, 1024, 72), (33, 1024, 72), (4, 8192, 160), (9, 4096, 160), (2, 12288, 64), (2, 100, 80),
