@@ -1172,7 +1172,8 @@ static int gemm_fp4(const void* x_codes, const void* w_codes, const F4Args& p, i
     // 4,096, 18.6 / 16.1 at 4,096 x 12,288; 400 rows 4.9 / 5.7 at 1,024 x 1,024, 9.8 / 9.1 at 4,096 x 4,096, 20.9 / 17.6 at 4,096 x
     // 12,288; with a gate 128 rows 15.3 / 17.0 at 24,576 x 4,096, 400 rows 9.8 / 10.6 at 4,096 x 4,096 and 42.7 / 25.1 at 24,576 x 4,096.
     const bool whole = EPI == 2 || (((uintptr_t)p.out | (size_t)p.ldc * (EPI == 0 ? 2 : 4)) & 31) == 0;
-    double clocks = few - (EPI == 2 ? 5500 : 3500);
+    // The kernel for a few tokens has its tiles of rows along the grid's second dimension, of which there are at most 65,535.
+    double clocks = p.T > 65535LL * F4_BM ? 1e300 : few - (EPI == 2 ? 5500 : 3500);
     for (int bn : {192, 256, 384}) {
       if (bn == 384 && EPI != 0) break;
       const double c = f4_pair_cost(p.T, p.N, p.K, bn, EPI, whole);

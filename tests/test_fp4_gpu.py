@@ -211,6 +211,28 @@ def test_product_at_sizes_of_prompts(rows, features, width):
         assert bool(((y.double() - want).abs() <= bound).all())
 
 
+def test_products_of_more_rows_than_a_grid_of_small_tiles_has():
+    """Over 65,535 tiles of 128 rows, narrow enough that small tiles would be the faster ones: the rows repeat 1,000 others."""
+    o, rows, width = ops(), 65535 * 128 + 1, 64
+    data = normal(1000, width, 1)
+    x, st = o.fp4_rows(rows, width, "cuda"), status()
+    o.fp4_quantise(data.cuda()[torch.arange(rows, device="cuda") % 1000], x)
+    w = held(normal(64, width, 2, False))[0]
+    some = held(data)[0]
+    want, want4 = torch.empty(1000, 64, dtype=torch.bfloat16, device="cuda"), o.fp4_rows(1000, 32, "cuda")
+    o.fp4_product(some, w, want, st)
+    o.fp4_gated_product(some, w, want4, st)
+    y, y4 = torch.empty(rows, 64, dtype=torch.bfloat16, device="cuda"), o.fp4_rows(rows, 32, "cuda")
+    o.fp4_product(x, w, y, st)
+    o.fp4_gated_product(x, w, y4, st)
+    assert int(st.item()) == 0
+    whole = rows // 1000 * 1000
+    for got, of in ((y, want), (y4.codes, want4.codes)):
+        assert bool((got[:whole].view(-1, 1000, got.shape[1]) == of).all()) and torch.equal(got[whole:], of[:rows - whole])
+    with pytest.raises(o.KernelSizeError):
+        o.fp4_product(x, w, y, st, form="few")
+
+
 @pytest.mark.parametrize("out", list(DT))
 @pytest.mark.parametrize("rows,features", [(1, 290), (40, 290), (300, 290), (300, 800)])
 @pytest.mark.parametrize("start,more", [(0, 30), (8, 46), (3, 11)])
