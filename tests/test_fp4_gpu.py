@@ -212,13 +212,14 @@ def test_product_at_sizes_of_prompts(rows, features, width):
 
 
 def test_products_of_more_rows_than_a_grid_of_small_tiles_has():
-    """Over 65,535 tiles of 128 rows, narrow enough that small tiles would be the faster ones: the rows repeat 1,000 others."""
+    """Over 65,535 tiles of 128 rows, narrow enough that small tiles would be the faster ones: the rows repeat 1,000 others, and hold
+    whole numbers of up to 4, whose sums are exact in any order."""
     o, rows, width = ops(), 65535 * 128 + 1, 64
-    data = normal(1000, width, 1)
+    g = torch.Generator().manual_seed(1)
+    data, weight = (torch.randint(-4, 5, (n, width), generator=g).float() for n in (1000, 64))
     x, st = o.fp4_rows(rows, width, "cuda"), status()
     o.fp4_quantise(data.cuda()[torch.arange(rows, device="cuda") % 1000], x)
-    w = held(normal(64, width, 2, False))[0]
-    some = held(data)[0]
+    w, some = held(weight)[0], held(data)[0]
     want, want4 = torch.empty(1000, 64, dtype=torch.bfloat16, device="cuda"), o.fp4_rows(1000, 32, "cuda")
     o.fp4_product(some, w, want, st)
     o.fp4_gated_product(some, w, want4, st)
