@@ -55,6 +55,8 @@ def _engine(args):
     if args.config_path:
         if not args.model_name:
             raise SystemExit("--config-path needs --model-name")
+        if args.feed_forward_weights:
+            raise SystemExit("--feed-forward-weights goes with --model, not with --config-path")
         return SyncEngine.from_config(args.config_path, args.model_name, log_interval=args.log_interval)
     if not args.model:
         raise SystemExit("give --model DIR or --config-path FILE --model-name NAME")

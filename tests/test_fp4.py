@@ -47,3 +47,11 @@ def test_bytes_in_a_wider_integer_type_are_read_as_bytes(wide):
     assert ops._fp4_bytes(own) is own
     other = ops.Fp4Rows(codes.float(), scales, 64)
     assert ops._fp4_bytes(other).codes.dtype is torch.float32
+
+
+def test_the_command_line_does_not_drop_the_option(tmp_path):
+    from qwen3_from_scratch_b200.cli import main
+    config = tmp_path / "batch.yaml"
+    config.write_text("models: []\n")
+    with pytest.raises(SystemExit, match="--feed-forward-weights"):
+        main(["generate", "--config-path", str(config), "--model-name", "a", "--feed-forward-weights", "fp4", "--prompt-ids", "1 2"])
