@@ -670,7 +670,7 @@ def test_sums_by_copies_are_given_up_cleanly(rows, features, width, drop):
 
 
 @pytest.mark.parametrize("drop", [0, 1])
-@pytest.mark.parametrize("rows,features,width", [(1, 200, 2816), (3, 200, 2816), (20, 136, 2816), (30, 48, 4352)])
+@pytest.mark.parametrize("rows,features,width", [(1, 208, 2816), (3, 208, 2816), (20, 144, 2816), (30, 48, 4352)])
 def test_sums_by_stores_are_given_up_cleanly(rows, features, width, drop):
     """Tiles whose sums go from block to block as stores, where all blocks give up or all but one of a single stage, which sends its
     sums to blocks that wait for more and waits itself for what never comes."""
