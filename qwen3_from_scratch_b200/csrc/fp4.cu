@@ -76,8 +76,9 @@ __device__ __forceinline__ void fp4_load_words(const T* row, int col, int K, con
   }
 }
 
-// What eight codes of a block with this scale stand for, as bfloat16 (every such value is one): the sizes by a table in two registers,
-// whose bytes a permutation picks by three bits of each code, times the scale, with the sign.
+// What eight codes of a block with this scale stand for, as bfloat16 (every such value is one, but for the 2^128 of a block that
+// reaches beyond 1.75 x 2^127: infinity): the sizes by a table in two registers, whose bytes a permutation picks by three bits of each
+// code, times the scale, with the sign.
 __device__ __forceinline__ void fp4_values8(uint32_t codes, uint32_t scale_byte, uint32_t (&out)[4]) {
   const uint32_t unit = scale_byte == 0u ? 0x0040u : scale_byte == 255u ? 0x7fc0u : scale_byte << 7;  // bits of 2^(b - 127)
   const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&(const uint32_t&)(unit * 0x10001u));

@@ -3212,7 +3212,8 @@ def fp4_quantise(x: torch.Tensor, out: Fp4Rows, values: Optional[torch.Tensor] =
     """Rounds the rows of x [T, K] (float32 or bfloat16; rows may lie further apart than K) into ``out``.  A block's scale is the
     smallest power of two X with max|x| <= 7 X; each x / X goes to the nearest value of the format, ties to the even code, and to
     +-6 beyond it.  A block that holds a value that is not finite gets the scale NaN.  ``values`` (float32 or bfloat16 [T, K],
-    contiguous): what the rows then stand for, exact in either type."""
+    contiguous): what the rows then stand for, exact in either type, except where a block reaches beyond 1.75 x 2^127: what is
+    rounded to 2^128 there, which neither type holds, is infinity."""
     if not x.is_cuda:
         raise KernelError(f"fp4_quantise.x: tensor is on {x.device}; the kernels run on the GPU only")
     T, K = x.shape if x.dim() == 2 else (0, 0)

@@ -121,6 +121,26 @@ def test_quantise_values_off_every_boundary(width, out):
         assert bool((room[:start] == 3).all()) and bool((room[start + 18 * width:] == 3).all()), start
 
 
+@pytest.mark.parametrize("out", list(DT))
+@pytest.mark.parametrize("dtype", list(DT))
+def test_quantise_values_of_the_largest_numbers(dtype, out):
+    """In a block that reaches beyond 1.75 x 2^127 values from there on are rounded to 4 x 2^126, which is no float: infinity with its
+    sign.  Everything else is exact."""
+    top = 2.0 ** 127
+    x = torch.zeros(3, 64)
+    x[0, :6] = torch.tensor([1.9921875, -1.9921875, 1.75, 1.5, -1.0, 0.125]) * top
+    x[1, :3] = torch.tensor([1.75, -1.75, 0.25]) * top  # 7 x 2^125
+    x[2, 32:34] = torch.tensor([-1.9921875, 0.5]) * top
+    x = x.to(DT[dtype])
+    assert bool(torch.isfinite(x).all())
+    r, values = junk_rows(3, 64), torch.empty(3, 64, dtype=DT[out], device="cuda")
+    ops().fp4_quantise(x.cuda(), r, values=values)
+    want = plain.rounded(x.double())
+    assert torch.equal(plain.read(r.codes, r.scales, 64)[0], want)
+    assert torch.equal(values.cpu().double(), want.float().double())
+    assert int(torch.isinf(values).sum()) == 4 and bool(torch.isfinite(values[1]).all())
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_quantise_what_is_not_finite(bad):
     x = normal(3, 100, 5)
