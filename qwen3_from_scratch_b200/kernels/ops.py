@@ -3272,6 +3272,13 @@ def fp4_add_rmsnorm(stream: torch.Tensor, delta: Optional[torch.Tensor], weight:
 FP4_FORMS = {None: 0, "few": 1, "pair192": 192, "pair256": 256, "pair384": 384}
 
 
+def _fp4_form(name: str, form: Optional[str]) -> int:
+    code = FP4_FORMS.get(form)
+    if code is None:
+        raise KernelError(f"{name}: no form {form!r} (there are {tuple(FP4_FORMS)})")
+    return code
+
+
 def fp4_product(x: Fp4Rows, w: Fp4Rows, out: torch.Tensor, status: torch.Tensor, form: Optional[str] = None) -> None:
     """out[T, N] = x[T, K] @ w[N, K]^T of rows held in four bits, accumulated in float32; out bfloat16 or float32, also a column
     view of a wider buffer.  ``form``: one of ``FP4_FORMS`` instead of the one that the sizes ask for (a few tokens' small tiles,
@@ -3286,7 +3293,7 @@ def fp4_product(x: Fp4Rows, w: Fp4Rows, out: torch.Tensor, status: torch.Tensor,
         raise KernelError(f"fp4_product: out {tuple(out.shape)} with strides {out.stride()} on {out.device} for {T} x {N}")
     code = library().q3_fp4_product(x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
                                     T, N, x.width, pitch if pitch > N else N, 1 if dtype_tag(out.dtype) == F32 else 0,
-                                    FP4_FORMS[form], status.data_ptr(), _stream())
+                                    _fp4_form("fp4_product", form), status.data_ptr(), _stream())
     if code:
         _done("fp4_product", code, f"T {T} N {N} K {x.width}")
 
@@ -3308,8 +3315,8 @@ def fp4_gated_product(x: Fp4Rows, w: Fp4Rows, out: Fp4Rows, status: torch.Tensor
     _check_fp4("fp4_gated_product.out", out, w.rows // 2, x.rows)
     code = library().q3_fp4_gated_product(x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(),
                                           out.codes.data_ptr(), out.scales.data_ptr(), x.rows, w.rows, x.width,
-                                          _fp4_gate("fp4_gated_product", activation), FP4_FORMS[form], status.data_ptr(),
-                                          _stream())
+                                          _fp4_gate("fp4_gated_product", activation), _fp4_form("fp4_gated_product", form),
+                                          status.data_ptr(), _stream())
     if code:
         _done("fp4_gated_product", code, f"T {x.rows} N {w.rows} K {x.width}")
 

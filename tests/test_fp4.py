@@ -55,3 +55,10 @@ def test_the_command_line_does_not_drop_the_option(tmp_path):
     config.write_text("models: []\n")
     with pytest.raises(SystemExit, match="--feed-forward-weights"):
         main(["generate", "--config-path", str(config), "--model-name", "a", "--feed-forward-weights", "fp4", "--prompt-ids", "1 2"])
+
+
+def test_an_unknown_form_is_refused():
+    from qwen3_from_scratch_b200.kernels import ops
+    assert [ops._fp4_form("p", f) for f in (None, "few", "pair384")] == [0, 1, 384]
+    with pytest.raises(ops.KernelError, match="no form 'pair128'"):
+        ops._fp4_form("p", "pair128")
