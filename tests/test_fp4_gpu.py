@@ -793,3 +793,165 @@ def test_products_of_bytes_in_a_wider_integer_type(rows, inner, width, wide):
         o.fp4_gated_product(x, gu, o.Fp4Rows(a.codes.to(wide), a.scales, inner), st)
     with pytest.raises(o.KernelError, match="uint8"):
         o.fp4_product(o.Fp4Rows(x.codes.float(), x.scales, width), gu, y, st)
+
+
+def test_feed_forward_of_a_prompt_is_its_parts():
+    """Where the rule takes pairs of CTAs for both products, several tiles each."""
+    for dtype in DT:
+        test_feed_forward_is_its_parts(dtype, 2100, 1024, 4104)
+
+
+# ---------------------------------------------------------------- models in bfloat16 and behind other norms
+def rms(t):
+    return float(t.double().square().mean().sqrt())
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("key", ["a", "b", "d"])
+def test_model_with_fp4_feed_forwards_in_bfloat16(tiny_folders, monkeypatch, key, graphs):
+    """The logits of a prompt and of single tokens, whole against whole.  Rounding to bfloat16 moves values across boundaries between
+    codes, so single logits may be off by a code's step; what is held is the root mean square over 60 positions, to 1.5 times what such
+    rounding does in the plain model (operands and results of the attention's projections, rotated heads, the feed-forward's result and
+    the head's operand).  A model without the rounding to four bits is further off than that."""
+    import plain_qwen3
+    from conftest import TINY, random_tokens
+    from qwen3_from_scratch_b200.engine.batch import Entry
+    from qwen3_from_scratch_b200.engine.session import Session
+    folder = tiny_folders[key]
+    cfg, w = plain_qwen3.read_model_folder(folder)
+    ids = random_tokens(TINY[key][0]["vocab_size"], 60, 3)
+    without = plain_qwen3.forward_logits(cfg, w, ids)
+    monkeypatch.setattr(plain_qwen3, "swiglu_mlp", plain_mlp)
+    want = plain_qwen3.forward_logits(cfg, w, ids)
+
+    def cut(t):
+        return t.to(torch.bfloat16).to(t.dtype)
+
+    rope, attend, mixer, head = (getattr(plain_qwen3, n) for n in ("apply_rope", "causal_attention", "self_attention", "lm_head"))
+    with monkeypatch.context() as m:
+        m.setattr(plain_qwen3, "apply_rope", lambda x, c, s: cut(rope(cut(x), c, s)))
+        m.setattr(plain_qwen3, "causal_attention", lambda q, k, v, window=None: cut(attend(q, k, cut(v), window)))
+        m.setattr(plain_qwen3, "self_attention", lambda x, *rest: cut(mixer(cut(x), *rest)))
+        m.setattr(plain_qwen3, "swiglu_mlp", lambda *rest: cut(plain_mlp(*rest)))
+        m.setattr(plain_qwen3, "lm_head", lambda h, *rest: head(cut(h), *rest))
+        noisy = plain_qwen3.forward_logits(cfg, w, ids)
+    bound = 1.5 * rms(noisy - want)
+    assert bound < 0.85 * rms(without - want)
+    session = Session(folder, dtype="bfloat16", page_size=16, num_pages=24, max_seqs=2, max_step_tokens=64, cuda_graphs=graphs,
+                      feed_forward_weights="fp4")
+    whole = session.step([Entry("r", ids, list(range(60)))]).float().cpu()
+    session.end("r")
+    rows = [session.step([Entry("s", [t], [0])]).float().cpu().clone() for t in ids]
+    session.check_status()
+    assert rms(whole - want) <= bound and rms(torch.cat(rows) - want) <= bound
+
+
+@pytest.mark.parametrize("key", ["a", "d"])
+def test_model_whose_feed_forwards_read_a_normed_sum(tiny_folders, monkeypatch, key):
+    """A block whose mixer leaves several terms norms them before the feed-forward, which then rounds the normed rows: in float32 the
+    logits of the same bound as above."""
+    import plain_qwen3
+    from conftest import TINY, random_tokens
+    from qwen3_from_scratch_b200.engine.batch import Entry
+    from qwen3_from_scratch_b200.engine.session import Session
+    from qwen3_from_scratch_b200.parts.base import PendingSum
+    from qwen3_from_scratch_b200.parts.mlp import GatedMLP
+    folder = tiny_folders[key]
+    cfg, w = plain_qwen3.read_model_folder(folder)
+    ids = random_tokens(TINY[key][0]["vocab_size"], 20, 3)
+    monkeypatch.setattr(plain_qwen3, "swiglu_mlp", plain_mlp)
+    want = plain_qwen3.forward_logits(cfg, w, ids).double()
+    session = Session(folder, dtype="float32", page_size=8, num_pages=16, max_seqs=2, max_step_tokens=64, feed_forward_weights="fp4",
+                      cuda_graphs=False)
+    for block in session.model.layers:
+        def two_terms(*args, forward=block.mixer.forward, **more):
+            a = forward(*args, **more)
+            return PendingSum.of(a, torch.zeros_like(a))
+        monkeypatch.setattr(block.mixer, "forward", two_terms)
+    calls = []
+    inner = GatedMLP._forward_fp4
+    monkeypatch.setattr(GatedMLP, "_forward_fp4", lambda self, x: calls.append(0) or inner(self, x))
+    whole = session.step([Entry("r", ids, list(range(20)))]).cpu().double()
+    session.end("r")
+    rows = [session.step([Entry("s", [t], [0])]).cpu().double() for t in ids]
+    session.check_status()
+    assert len(calls) == len(session.model.layers) * 21
+    for got in (whole, torch.cat(rows)):
+        assert float((got - want).abs().max()) <= 1e-4 * float(want.abs().max())
+
+
+def plain_relu_glu(x, w, p):
+    """The feed-forward of the plain Binupel with weights and activations rounded."""
+    h = plain.rounded(x)
+    a = plain.rounded(torch.relu(h @ plain.rounded(w[p + "gate"]).t()) * (h @ plain.rounded(w[p + "up"]).t()))
+    return a @ plain.rounded(w[p + "down"]).t()
+
+
+@pytest.mark.parametrize("key", ["p", "q", "r"])
+def test_post_norm_model_with_fp4_feed_forwards(tmp_path, monkeypatch, key):
+    """Binupel, whose norms stand behind the sums and whose gates are ReLU: float32, a prompt whole and token by token.  In the plain
+    model a disturbance of 2e-6 of the embeddings moves no code at these tokens (six drawn), so the bound is that of the model above."""
+    import plain_binupel
+    from binupel_models import CONFIGS, make_folder
+    from qwen3_from_scratch_b200.engine.batch import Entry
+    from qwen3_from_scratch_b200.engine.session import Session
+    folder = make_folder(str(tmp_path), *CONFIGS[key])
+    cfg, w = plain_binupel.read_model_folder(folder)
+    ids = torch.randint(0, cfg["vocab"], (20,), generator=torch.Generator().manual_seed(3)).tolist()
+    without = plain_binupel.forward_logits(cfg, w, ids)
+    monkeypatch.setattr(plain_binupel, "relu_glu", plain_relu_glu)
+    want = plain_binupel.forward_logits(cfg, w, ids)
+    session = Session(folder, dtype="float32", page_size=8, num_pages=16, max_seqs=2, max_step_tokens=64, feed_forward_weights="fp4")
+    whole = session.step([Entry("r", ids, list(range(20)))]).cpu().double()
+    session.end("r")
+    rows = [session.step([Entry("s", [t], [0])]).cpu().double() for t in ids]
+    session.check_status()
+    scale = float(want.abs().max())
+    for got in (whole, torch.cat(rows)):
+        assert float((got - want).abs().max()) <= 1e-4 * scale
+    assert float((without - want).abs().max()) > 1e-3 * scale
+
+
+@pytest.mark.parametrize("act", ["silu", "relu", "gelu_tanh"])
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_gated_feed_forward_of_normed_rows(rows, dtype, act):
+    """The part by itself, given rows that are normed already: every result is a sum of what the gate may have left (both ends of each
+    value's range) times the weight, rounded once."""
+    from qwen3_from_scratch_b200.parts.base import PartSpec, Runtime
+    from qwen3_from_scratch_b200.registry import create_part
+    width, inner = 136, 264
+    part = create_part("feed_forward", PartSpec("gated_mlp", {"hidden_size": width, "intermediate_size": inner, "activation": act}), name="f")
+    g = torch.Generator().manual_seed(4)
+    stored = {n: (torch.randn(s, generator=g) * s[1] ** -0.5).to(torch.bfloat16)
+              for n, s in (("gate", (inner, width)), ("up", (inner, width)), ("down", (width, inner)))}
+    x = normal(rows, width, rows).to(DT[dtype])
+    rt = Runtime(torch.device("cuda:0"), DT[dtype], 320, 2, feed_forward_weights="fp4")
+    part.setup(rt, {f"f.{n}_proj.weight": t.to(DT[dtype]).cuda() for n, t in stored.items()})
+    got = part.forward(x.cuda()).cpu()
+    assert got.dtype == DT[dtype] and got.shape == x.shape and int(rt.status.item()) == 0
+    gate, up, down = (plain.rounded(stored[n].double()) for n in ("gate", "up", "down"))
+    a, slack = gated_bounds(plain.rounded(x.double()), interleaved(gate, up), act)
+    low, high = plain.between(a, slack)
+    middle, reach = (low + high) / 2, (high - low) / 2
+    want, tol = middle @ down.t(), reach @ down.abs().t() + product_tolerance(middle.abs() + reach, down)
+    if dtype == "bfloat16":
+        tol = tol + (want.abs() + tol) * 2.0 ** -8
+    assert bool(((got.double() - want).abs() <= tol).all())
+    assert float((reach > 0).double().mean()) < 0.01  # the ranges hardly ever hold two values
+
+
+# ---------------------------------------------------------------- the stream that every operator asks for
+def test_the_stream_handle_is_torchs_current_one():
+    import threading
+    o, side = ops(), torch.cuda.Stream()
+    torch.zeros(1, device="cuda")
+    assert o._stream() == torch.cuda.current_stream().cuda_stream
+    with torch.cuda.stream(side):
+        assert o._stream() == side.cuda_stream == torch.cuda.current_stream().cuda_stream
+        seen = []
+        thread = threading.Thread(target=lambda: seen.append((o._stream(), torch.cuda.current_stream().cuda_stream)))
+        thread.start()
+        thread.join()
+        assert len(seen) == 1 and seen[0][0] == seen[0][1]
+    assert o._stream() == torch.cuda.current_stream().cuda_stream != side.cuda_stream
