@@ -304,8 +304,8 @@ __device__ __forceinline__ void f4_gated_block(const uint32_t (&v0)[32], const u
 // are chosen (f4_few_shape) to give each SM one block.
 //
 // The blocks of a cluster send each row of sums, by asynchronous stores that the receiver's mbarrier counts, to the block that
-// finishes that row (rank r % split).  No block reads another's memory, so none has to stay for the others: a barrier of the
-// whole cluster behind the reading took 1.1 us.  The stores take some two clocks per 16 bytes; above 8,000 results of a tile a row
+// finishes that row (rank r % split).  No block reads another's memory, so none has to stay for the others but one whose own wait
+// for sums runs out: a barrier of the whole cluster behind the reading took 1.1 us.  The stores take some two clocks per 16 bytes; above 8,000 results of a tile a row
 // goes as one bulk copy from shared memory instead, and the blocks stay for each other (by then with an arrival that waits for no
 // stores): 128 x 4,096 x 12,288 11.8 us by stores and 10.2 by copies, 64 rows 9.2 and 8.5, but 64 x 4,096 x 4,096 in tiles of 64
 // 6.1 and 6.4.
